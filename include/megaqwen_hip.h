@@ -276,6 +276,86 @@ int mq_flash_attn_bhwd_nows(const void* d_q, const void* d_k, const void* d_v, v
                             int batch, int heads, int seq_len, int head_dim, int dtype,
                             float scale, void* stream);
 
+/* ---- 4-bit weights, a 4-bit key/value cache and log probabilities.  The reference's W4 and
+ * quantised-cache features belong to its split-GEMM backend; these have their own formats, given
+ * here.  None of them needs a decoder, keeps anything between calls or allocates; every one is
+ * asynchronous on `stream` and may be captured into a HIP graph.  Outputs must not overlap inputs
+ * unless said otherwise.
+ *
+ * A code u (0..15) stands for scale * (u - zero); a byte holds two codes, the even element in its
+ * low half. */
+#define MQ_DTYPE_F32 2
+
+/* out[m][n] = sum_k x[m][k] * w[n][k] (+ residual[m][n]), m < rows, with 4-bit weights in groups of
+ * `group_size` (32, 64 or 128, dividing k) along k:
+ *   w[n][k] = scales[n][k / group_size] * (u[n][k] - zeros[n][k / group_size]).
+ * x: contiguous [rows, k], x_dtype MQ_DTYPE_BF16 or MQ_DTYPE_F16, 16-byte aligned.  qweight: bytes
+ * [n, k / 2], 16-byte aligned.  scales: [n, k / group_size] of scale_dtype (BF16 or F16).  zeros:
+ * bytes [n, k / group_size], or NULL for 8 everywhere.  residual (NULL for none; it may be out
+ * itself) and out: contiguous [rows, n] of out_dtype: x_dtype or MQ_DTYPE_F32.  Sums in fp32,
+ * rounded to nearest-even once.  rows == 0 or n == 0 is a no-op. */
+int mq_w4_linear(const void* d_x, const void* d_qweight, const void* d_scales, const void* d_zeros,
+                 const void* d_residual, void* d_out, int rows, int n, int k, int group_size,
+                 int x_dtype, int scale_dtype, int out_dtype, void* stream);
+
+/* A key/value cache in 4 bits, caller-owned: codes as bytes [batch, kv_heads, max_seq, head_dim / 2]
+ * for keys and for values (zero is 8), and bf16 scales [batch, kv_heads, max_seq, 2,
+ * head_dim / group_size] (a position's key scales, then its value scales).  head_dim is 64 or 128,
+ * group_size 32, 64 or 128 (at most head_dim); codes 16-byte and scales 4-byte aligned.
+ * Every call works on the last `t` positions of every sequence: lengths (device memory, int32
+ * [batch]) counts a sequence's positions with these, so that row i of t is at position
+ * lengths[b] - t + i.  A position outside [0, max_seq) is left out, so a batch of unequal lengths
+ * is padded at its front; whatever lengths holds, nothing outside the tensors is accessed. */
+typedef struct mq_kv4_cache {
+  void* k_codes;
+  void* v_codes;
+  void* scales;
+  int batch;
+  int kv_heads;
+  int max_seq;
+  int head_dim;
+  int group_size;
+} mq_kv4_cache;
+/* Quantises t key and value rows per sequence: scale = bf16(max |x| / 7) of a group, u = 8 +
+ * clamp(round-to-even(x / scale), -7, 7).  A group of zeros has scale 0 and codes 8; one that holds
+ * an infinity or a NaN has scale NaN (all its values read as NaN).  d_k, d_v: [batch, t, kv_heads,
+ * head_dim] of dtype (BF16 or F16) with the last dimension contiguous; k_strides and v_strides: host
+ * arrays of the element strides of the first three dimensions (>= 0). */
+int mq_kv4_append(const mq_kv4_cache* cache, const void* d_k, const int64_t* k_strides,
+                  const void* d_v, const int64_t* v_strides, const int32_t* d_lengths, int t,
+                  int dtype, void* stream);
+/* The values that those rows stand for, rounded to out_dtype (BF16, F16 or F32, which holds them
+ * exactly): contiguous [batch, t, kv_heads, head_dim]; rows that do not exist are 0. */
+int mq_kv4_read(const mq_kv4_cache* cache, const int32_t* d_lengths, int t, void* d_k_out,
+                void* d_v_out, int out_dtype, void* stream);
+/* Attention over the cache: query row i of sequence b looks at positions 0 .. lengths[b] - t + i,
+ *   out[b][i][h] = sum_p softmax_p(scale * q[b][i][h] . k[b][hk][p]) v[b][hk][p],
+ * hk = h / (q_heads / kv_heads); a row that has no position to look at gives 0.  max_len bounds the
+ * positions that are looked at (lengths above it are cut to it) and decides how the work is split;
+ * max_seq is always right.  d_q: [batch, t, q_heads, head_dim] of dtype with element strides
+ * q_strides as above; out: contiguous, of the same type.  fp32 scores, softmax and sums.
+ * d_workspace: mq_kv4_attend_workspace_bytes() bytes, 16-byte aligned (NULL if that is 0); calls
+ * that may overlap need one each. */
+size_t mq_kv4_attend_workspace_bytes(const mq_kv4_cache* cache, int t, int q_heads, int max_len);
+int mq_kv4_attend(const mq_kv4_cache* cache, const void* d_q, const int64_t* q_strides,
+                  const int32_t* d_lengths, int t, int q_heads, int max_len, int dtype, float scale,
+                  void* d_out, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* For each row of logits (dtype BF16, F16 or F32; rows row_stride elements apart): the log
+ * probability (nats) of its token, the entropy of its distribution and, if top_k > 0 (at most
+ * 32 and vocab), its top_k most likely tokens in falling order with their log probabilities; equal
+ * logits are ordered by the lower token.  d_tokens: int32, or int64 if tokens_are_64bit.  A token
+ * outside [0, vocab) has log probability -inf, as has one whose logit is -inf.  A row of -inf alone
+ * has no distribution: log probabilities -inf, entropy 0, tokens 0 .. top_k - 1.  A row that holds a
+ * NaN or +inf gives NaN log probabilities and entropy (its top tokens are in the order of their
+ * logits, or 0 .. top_k - 1 if it holds a NaN).  fp32 outputs [rows], [rows], [rows, top_k] and
+ * int32 [rows, top_k].  d_workspace as above. */
+size_t mq_token_logprobs_workspace_bytes(int rows, int vocab, int top_k);
+int mq_token_logprobs(const void* d_logits, int64_t row_stride, const void* d_tokens,
+                      int tokens_are_64bit, float* d_logprobs, float* d_entropy,
+                      float* d_top_logprobs, int32_t* d_top_tokens, int rows, int vocab, int top_k,
+                      int dtype, void* d_workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,7 @@ MQ_MODE_PERSISTENT = 0
 MQ_MODE_MULTI_KERNEL = 1
 MQ_DTYPE_BF16 = 0
 MQ_DTYPE_F16 = 1
+MQ_DTYPE_F32 = 2
 
 # Every symbol include/megaqwen_hip.h declares (tests check the library exports all of them).
 EXPORTED = (
@@ -33,6 +34,8 @@ EXPORTED = (
     "mq_op_mlp", "mq_op_decode_layer", "mq_op_lm_head", "mq_flash_attn_workspace_bytes",
     "mq_flash_attn_bhwd", "mq_flash_attn_bhwd_nows", "mq_exchange_epoch", "mq_exchange_epoch_advance", "mq_exchange_tag",
     "mq_exchange_epoch_period", "mq_debug_set_exchange_epoch", "mq_debug_get_exchange_epoch",
+    "mq_w4_linear", "mq_kv4_append", "mq_kv4_read", "mq_kv4_attend_workspace_bytes", "mq_kv4_attend",
+    "mq_token_logprobs_workspace_bytes", "mq_token_logprobs",
 )
 
 
@@ -52,6 +55,12 @@ class ModelDesc(ctypes.Structure):
         ("lm_head", ctypes.c_void_p), ("cos_table", ctypes.c_void_p),
         ("sin_table", ctypes.c_void_p), ("layers", ctypes.POINTER(LayerWeights)),
     ]
+
+
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("scales", ctypes.c_void_p), ("batch", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("max_seq", ctypes.c_int), ("head_dim", ctypes.c_int), ("group_size", ctypes.c_int)]
 
 
 class MegaQwenError(RuntimeError):
@@ -111,6 +120,13 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         "mq_exchange_epoch_period": (U32, []),
         "mq_debug_set_exchange_epoch": (I, [P, U32, P]),
         "mq_debug_get_exchange_epoch": (I, [P, ctypes.POINTER(U32), P]),
+        "mq_w4_linear": (I, [P, P, P, P, P, P, I, I, I, I, I, I, I, P]),
+        "mq_kv4_append": (I, [P, P, P, P, P, P, I, I, P]),
+        "mq_kv4_read": (I, [P, P, I, P, P, I, P]),
+        "mq_kv4_attend_workspace_bytes": (S, [P, I, I, I]),
+        "mq_kv4_attend": (I, [P, P, P, P, I, I, I, I, ctypes.c_float, P, P, S, P]),
+        "mq_token_logprobs_workspace_bytes": (S, [I, I, I]),
+        "mq_token_logprobs": (I, [P, ctypes.c_int64, P, I, P, P, P, P, I, I, I, I, P, S, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -17,7 +17,9 @@
 #include "../../include/megaqwen_hip.h"
 #include "mq_decode.h"
 #include "mq_flash.h"
+#include "mq_logprobs.h"
 #include "mq_prefill.h"
+#include "mq_q4.h"
 
 namespace {
 
@@ -664,6 +666,202 @@ int mq_flash_attn_bhwd_nows(const void* d_q, const void* d_k, const void* d_v, v
   const int rc = check_flash_attn(d_q, d_k, d_v, d_out, batch, heads, seq_len, head_dim, dtype, &run);
   if (rc != MQ_OK || !run) return rc;
   return launch_flash_attn(d_q, d_k, d_v, d_out, batch, heads, seq_len, dtype, scale, stream);
+}
+
+// ---- 4-bit weights, the 4-bit key/value cache and log probabilities
+
+static bool is16(int dtype) { return dtype == MQ_DTYPE_BF16 || dtype == MQ_DTYPE_F16; }
+static size_t dtype_bytes(int dtype) { return dtype == MQ_DTYPE_F32 ? 4 : 2; }
+static bool ranges_overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const char* x = static_cast<const char*>(a);
+  const char* y = static_cast<const char*>(b);
+  return x != nullptr && y != nullptr && x < y + nb && y < x + na;
+}
+static int launch_result(int rc) {
+  return rc == 0 ? MQ_OK : fail(MQ_ERR_HIP, "launch failed (%s)", hipGetErrorString(hipGetLastError()));
+}
+
+int mq_w4_linear(const void* d_x, const void* d_qweight, const void* d_scales, const void* d_zeros,
+                 const void* d_residual, void* d_out, int rows, int n, int k, int group_size,
+                 int x_dtype, int scale_dtype, int out_dtype, void* stream) {
+  if (rows < 0 || n < 0 || k < 1)
+    return fail(MQ_ERR_INVALID_ARG, "bad size (rows %d, n %d, k %d)", rows, n, k);
+  if (group_size != 32 && group_size != 64 && group_size != 128)
+    return fail(MQ_ERR_INVALID_ARG, "group_size %d is not 32, 64 or 128", group_size);
+  if (k % group_size != 0)
+    return fail(MQ_ERR_INVALID_ARG, "k = %d is not a multiple of group_size %d", k, group_size);
+  if (!is16(x_dtype) || !is16(scale_dtype) || (out_dtype != x_dtype && out_dtype != MQ_DTYPE_F32))
+    return fail(MQ_ERR_INVALID_ARG, "unsupported types (x %d, scales %d, out %d)", x_dtype,
+                scale_dtype, out_dtype);
+  if (rows == 0 || n == 0) return MQ_OK;
+  if (d_x == nullptr || d_qweight == nullptr || d_scales == nullptr || d_out == nullptr)
+    return fail(MQ_ERR_INVALID_ARG, "NULL argument");
+  if (!aligned16(d_x) || !aligned16(d_qweight))
+    return fail(MQ_ERR_INVALID_ARG, "x and qweight must be 16-byte aligned");
+  const size_t groups = (size_t)n * (k / group_size);
+  const size_t out_bytes = (size_t)rows * n * dtype_bytes(out_dtype);
+  if (ranges_overlap(d_out, out_bytes, d_x, (size_t)rows * k * 2) ||
+      ranges_overlap(d_out, out_bytes, d_qweight, (size_t)n * (k / 2)) ||
+      ranges_overlap(d_out, out_bytes, d_scales, groups * 2) ||
+      ranges_overlap(d_out, out_bytes, d_zeros, groups) ||
+      (d_residual != d_out && ranges_overlap(d_out, out_bytes, d_residual, out_bytes)))
+    return fail(MQ_ERR_INVALID_ARG, "out must not overlap an input");
+  const MqW4Args a = {static_cast<const uint16_t*>(d_x), static_cast<const uint8_t*>(d_qweight),
+                      static_cast<const uint16_t*>(d_scales), static_cast<const uint8_t*>(d_zeros),
+                      d_residual, d_out, rows, n, k, group_size, x_dtype, scale_dtype, out_dtype};
+  return launch_result(mq_launch_w4_linear(a, static_cast<hipStream_t>(stream)));
+}
+
+// Checks shared by the cache's entry points.  *run is false for an empty problem.
+static int check_kv4(const mq_kv4_cache* c, const int32_t* d_lengths, int t, MqKv4* out, bool* run) {
+  *run = false;
+  if (c == nullptr) return fail(MQ_ERR_INVALID_ARG, "cache is NULL");
+  if (c->batch < 0 || c->kv_heads < 1 || c->max_seq < 1 || t < 0)
+    return fail(MQ_ERR_INVALID_ARG, "bad size (batch %d, kv_heads %d, max_seq %d, t %d)", c->batch,
+                c->kv_heads, c->max_seq, t);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(MQ_ERR_INVALID_ARG, "head_dim %d is not 64 or 128", c->head_dim);
+  const int g = c->group_size;
+  if ((g != 32 && g != 64 && g != 128) || g > c->head_dim)
+    return fail(MQ_ERR_INVALID_ARG, "group_size %d is not 32, 64 or 128, at most head_dim", g);
+  if (c->batch > 65535 || (long long)c->batch * t * c->kv_heads > (1ll << 28))
+    return fail(MQ_ERR_INVALID_ARG, "too many rows (batch %d, t %d, kv_heads %d)", c->batch, t, c->kv_heads);
+  if (c->batch == 0 || t == 0) return MQ_OK;
+  if (c->k_codes == nullptr || c->v_codes == nullptr || c->scales == nullptr || d_lengths == nullptr)
+    return fail(MQ_ERR_INVALID_ARG, "NULL argument");
+  if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || (reinterpret_cast<uintptr_t>(c->scales) & 3u))
+    return fail(MQ_ERR_INVALID_ARG, "codes must be 16-byte and scales 4-byte aligned");
+  *out = MqKv4{static_cast<uint8_t*>(c->k_codes), static_cast<uint8_t*>(c->v_codes),
+               static_cast<uint16_t*>(c->scales), d_lengths, c->batch, t, c->kv_heads, c->head_dim,
+               c->max_seq, g};
+  *run = true;
+  return MQ_OK;
+}
+
+static int check_strides(const int64_t* s, const char* name, MqStrides* out) {
+  if (s == nullptr) return fail(MQ_ERR_INVALID_ARG, "%s strides are NULL", name);
+  if (s[0] < 0 || s[1] < 0 || s[2] < 0) return fail(MQ_ERR_INVALID_ARG, "negative %s stride", name);
+  *out = MqStrides{s[0], s[1], s[2]};
+  return MQ_OK;
+}
+
+int mq_kv4_append(const mq_kv4_cache* cache, const void* d_k, const int64_t* k_strides,
+                  const void* d_v, const int64_t* v_strides, const int32_t* d_lengths, int t,
+                  int dtype, void* stream) {
+  MqKv4 c;
+  MqStrides ks, vs;
+  bool run;
+  int rc = check_kv4(cache, d_lengths, t, &c, &run);
+  if (rc != MQ_OK) return rc;
+  if (!is16(dtype))
+    return fail(MQ_ERR_INVALID_ARG, "dtype %d is neither MQ_DTYPE_BF16 nor MQ_DTYPE_F16", dtype);
+  if (!run) return MQ_OK;
+  if ((rc = check_strides(k_strides, "k", &ks)) != MQ_OK) return rc;
+  if ((rc = check_strides(v_strides, "v", &vs)) != MQ_OK) return rc;
+  if (d_k == nullptr || d_v == nullptr) return fail(MQ_ERR_INVALID_ARG, "NULL argument");
+  return launch_result(mq_launch_kv4_append(c, static_cast<const uint16_t*>(d_k), ks,
+                                            static_cast<const uint16_t*>(d_v), vs,
+                                            dtype == MQ_DTYPE_F16, static_cast<hipStream_t>(stream)));
+}
+
+int mq_kv4_read(const mq_kv4_cache* cache, const int32_t* d_lengths, int t, void* d_k_out,
+                void* d_v_out, int out_dtype, void* stream) {
+  MqKv4 c;
+  bool run;
+  const int rc = check_kv4(cache, d_lengths, t, &c, &run);
+  if (rc != MQ_OK) return rc;
+  if (!is16(out_dtype) && out_dtype != MQ_DTYPE_F32)
+    return fail(MQ_ERR_INVALID_ARG, "unsupported output type %d", out_dtype);
+  if (!run) return MQ_OK;
+  if (d_k_out == nullptr || d_v_out == nullptr || !aligned16(d_k_out) || !aligned16(d_v_out))
+    return fail(MQ_ERR_INVALID_ARG, "outputs must be non-NULL and 16-byte aligned");
+  return launch_result(mq_launch_kv4_read(c, d_k_out, d_v_out, out_dtype, static_cast<hipStream_t>(stream)));
+}
+
+// Sizes of an attend call, beyond those of check_kv4.
+static int check_attend(const mq_kv4_cache* c, int t, int q_heads, int max_len) {
+  if (q_heads < 1 || q_heads % c->kv_heads != 0)
+    return fail(MQ_ERR_INVALID_ARG, "q_heads %d is not a multiple of kv_heads %d", q_heads, c->kv_heads);
+  if (max_len < 1 || max_len > c->max_seq)
+    return fail(MQ_ERR_INVALID_ARG, "max_len %d outside [1, max_seq=%d]", max_len, c->max_seq);
+  if ((long long)t * q_heads > (1 << 24) || (long long)c->batch * t * q_heads > (1ll << 28))
+    return fail(MQ_ERR_INVALID_ARG, "too many query rows (batch %d, t %d, q_heads %d)", c->batch, t, q_heads);
+  return MQ_OK;
+}
+
+size_t mq_kv4_attend_workspace_bytes(const mq_kv4_cache* cache, int t, int q_heads, int max_len) {
+  if (cache == nullptr || cache->kv_heads < 1 || cache->batch < 1 || t < 1 ||
+      check_attend(cache, t, q_heads, max_len) != MQ_OK)
+    return 0;
+  return mq_kv4_attend_workspace(cache->batch, t, q_heads, cache->kv_heads, cache->head_dim,
+                                 cache->group_size, max_len);
+}
+
+int mq_kv4_attend(const mq_kv4_cache* cache, const void* d_q, const int64_t* q_strides,
+                  const int32_t* d_lengths, int t, int q_heads, int max_len, int dtype, float scale,
+                  void* d_out, void* d_workspace, size_t workspace_bytes, void* stream) {
+  MqKv4 c;
+  MqStrides qs;
+  bool run;
+  int rc = check_kv4(cache, d_lengths, t, &c, &run);
+  if (rc != MQ_OK) return rc;
+  if ((rc = check_attend(cache, t, q_heads, max_len)) != MQ_OK) return rc;
+  if (!is16(dtype))
+    return fail(MQ_ERR_INVALID_ARG, "dtype %d is neither MQ_DTYPE_BF16 nor MQ_DTYPE_F16", dtype);
+  if (!run) return MQ_OK;
+  if ((rc = check_strides(q_strides, "q", &qs)) != MQ_OK) return rc;
+  if (d_q == nullptr || d_out == nullptr || !aligned16(d_out))
+    return fail(MQ_ERR_INVALID_ARG, "q and out must be non-NULL, out 16-byte aligned");
+  const size_t out_bytes = (size_t)c.B * t * q_heads * c.D * 2;
+  const size_t q_bytes = 2 * ((size_t)(c.B - 1) * qs.b + (size_t)(t - 1) * qs.t + (size_t)(q_heads - 1) * qs.h + c.D);
+  const size_t code_bytes = (size_t)c.B * c.Hkv * c.S * (c.D / 2);
+  if (ranges_overlap(d_out, out_bytes, d_q, q_bytes) || ranges_overlap(d_out, out_bytes, c.kq, code_bytes) ||
+      ranges_overlap(d_out, out_bytes, c.vq, code_bytes) ||
+      ranges_overlap(d_out, out_bytes, c.scales, code_bytes * 8 / c.G))
+    return fail(MQ_ERR_INVALID_ARG, "out must not overlap q or the cache");
+  const size_t ws = mq_kv4_attend_workspace(c.B, t, q_heads, c.Hkv, c.D, c.G, max_len);
+  if (ws > 0 && (d_workspace == nullptr || workspace_bytes < ws || !aligned16(d_workspace)))
+    return fail(MQ_ERR_INVALID_ARG, "workspace needs %zu bytes, 16-byte aligned (got %zu)", ws, workspace_bytes);
+  const float scale_log2 = (float)((double)scale * 1.4426950408889634);
+  return launch_result(mq_launch_kv4_attend(c, static_cast<const uint16_t*>(d_q), qs,
+                                            static_cast<uint16_t*>(d_out), q_heads, max_len,
+                                            dtype == MQ_DTYPE_F16, scale_log2, d_workspace,
+                                            static_cast<hipStream_t>(stream)));
+}
+
+static int check_logprobs(int rows, int vocab, int top_k) {
+  if (rows < 0 || vocab < 1) return fail(MQ_ERR_INVALID_ARG, "bad size (rows %d, vocab %d)", rows, vocab);
+  if (top_k < 0 || top_k > MQ_TOP_MAX || top_k > vocab)
+    return fail(MQ_ERR_INVALID_ARG, "top_k %d outside [0, min(%d, vocab=%d)]", top_k, MQ_TOP_MAX, vocab);
+  return MQ_OK;
+}
+
+size_t mq_token_logprobs_workspace_bytes(int rows, int vocab, int top_k) {
+  if (check_logprobs(rows, vocab, top_k) != MQ_OK || rows == 0) return 0;
+  return mq_logprobs_workspace(rows, vocab, top_k);
+}
+
+int mq_token_logprobs(const void* d_logits, int64_t row_stride, const void* d_tokens,
+                      int tokens_are_64bit, float* d_logprobs, float* d_entropy,
+                      float* d_top_logprobs, int32_t* d_top_tokens, int rows, int vocab, int top_k,
+                      int dtype, void* d_workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_logprobs(rows, vocab, top_k);
+  if (rc != MQ_OK) return rc;
+  if (!is16(dtype) && dtype != MQ_DTYPE_F32)
+    return fail(MQ_ERR_INVALID_ARG, "unsupported type %d", dtype);
+  if (row_stride < 0) return fail(MQ_ERR_INVALID_ARG, "negative row_stride");
+  if (rows == 0) return MQ_OK;
+  if (d_logits == nullptr || d_tokens == nullptr || d_logprobs == nullptr || d_entropy == nullptr ||
+      (top_k > 0 && (d_top_logprobs == nullptr || d_top_tokens == nullptr)))
+    return fail(MQ_ERR_INVALID_ARG, "NULL argument");
+  if (reinterpret_cast<uintptr_t>(d_logits) % dtype_bytes(dtype) != 0)
+    return fail(MQ_ERR_INVALID_ARG, "logits are not aligned to their type");
+  const size_t ws = mq_logprobs_workspace(rows, vocab, top_k);
+  if (ws > 0 && (d_workspace == nullptr || workspace_bytes < ws || !aligned16(d_workspace)))
+    return fail(MQ_ERR_INVALID_ARG, "workspace needs %zu bytes, 16-byte aligned (got %zu)", ws, workspace_bytes);
+  const MqLogprobArgs a = {d_logits, d_tokens, d_logprobs, d_entropy, d_top_logprobs, d_top_tokens,
+                           (long long)row_stride, rows, vocab, top_k, dtype, tokens_are_64bit != 0};
+  return launch_result(mq_launch_token_logprobs(a, d_workspace, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -11,7 +11,7 @@
   `reset()`, `position()`, `get_k_cache()`, `get_v_cache()`.
 
 Both also expose `decode_step_with_logits(int) -> (int, fp32[vocab])`, the per-step logits hook
-of chat.py's `decode_ldg_with_logits` (chat.py:241-314).
+of chat.py's `decode_ldg_with_logits` (chat.py:241-314), and `decode_step_with_logprobs(int, top_k)`.
 
 The KV caches and the workspace are torch tensors owned by the Python object (the reference's
 C++ object owns its caches, bindings_decode.cpp:127-158); the library handle only points at
@@ -24,6 +24,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .logprobs import MAX_TOP_K, token_logprobs
 from .spec import COMPILED_LAYER_SHAPE
 
 _NKV, _D = COMPILED_LAYER_SHAPE["num_kv_heads"], COMPILED_LAYER_SHAPE["head_dim"]
@@ -154,6 +155,20 @@ class MegakernelDecoder:
         _lib.check(self._lib.mq_decode_step(self._h, self._tok.data_ptr(), self._tok.data_ptr() + 4,
                                             self._logits.data_ptr(), _stream_ptr()))
         return int(self._tok[1].item()), self._logits.clone()
+
+    def decode_step_with_logprobs(self, input_token_id: int, top_k: int = 0):
+        """One greedy step: (next token, TokenLogprobs of it): its log probability, the entropy of the
+        step's distribution and its top_k (at most 32) most likely tokens, fp32/int32 CUDA tensors
+        of one row (megaqwen_amd.logprobs)."""
+        if not 0 <= int(top_k) <= min(MAX_TOP_K, self.vocab_size):
+            raise ValueError(f"top_k must be in [0, min({MAX_TOP_K}, vocab={self.vocab_size})], got {top_k}")
+        if self._logits is None:
+            self._logits = torch.empty(self.vocab_size, dtype=torch.float32, device=self._tok.device)
+        self._tok[0].fill_(self._check_token(input_token_id))
+        _lib.check(self._lib.mq_decode_step(self._h, self._tok.data_ptr(), self._tok.data_ptr() + 4,
+                                            self._logits.data_ptr(), _stream_ptr()))
+        r = token_logprobs(self._logits, self._tok[1], top_k=top_k)
+        return int(self._tok[1].item()), r
 
     def debug_decode_step_layers(self, input_token_id: int):
         """(next token, fp32 logits [vocab], hidden state after every layer [num_layers, H]);

@@ -90,6 +90,28 @@ def decoder_last_logits(decoder, input_ids: Sequence[int]) -> torch.Tensor:
     return logits.float().cpu()
 
 
+def decoder_logprobs(decoder, input_ids: Sequence[int], top_k: int = 0):
+    """TokenLogprobs of input_ids[1:], each given the tokens before it: row i is for input_ids[i + 1]
+    (its log probability, the entropy of the distribution it came from and the top_k most likely
+    tokens).  Every token but the last is decoded at its position, with logits."""
+    from .logprobs import TokenLogprobs, token_logprobs
+    ids = [int(t) for t in input_ids]
+    if len(ids) < 2:
+        raise ValueError("at least two tokens are needed")
+    decoder.reset()
+    rows = []
+    for t, nxt in zip(ids[:-1], ids[1:]):
+        _, logits = decoder.decode_step_with_logits(t)
+        rows.append(token_logprobs(logits, torch.tensor(nxt, device=logits.device), top_k=top_k))
+    return TokenLogprobs(*(torch.stack(x) for x in zip(*rows)))
+
+
+def decoder_perplexity(decoder, input_ids: Sequence[int]) -> float:
+    """exp(mean next-token NLL) of the tokens under the decoder, as perplexity_from_logits computes it
+    from a whole sequence's logits."""
+    return float(torch.exp(-decoder_logprobs(decoder, input_ids).logprobs.mean()))
+
+
 def evaluate(name: str, decoder, prompt_ids: Sequence[Sequence[int]],
              ref_logits: Sequence[torch.Tensor]) -> QualityResult:
     """Mean KL(P_ref || P_decoder) and argmax agreement over prompts (quality_metrics.py:214-233).
