@@ -719,6 +719,7 @@ static int check_kv4(const mq_kv4_cache* c, const int32_t* d_lengths, int t, MqK
   if (c->batch < 0 || c->kv_heads < 1 || c->max_seq < 1 || t < 0)
     return fail(MQ_ERR_INVALID_ARG, "bad size (batch %d, kv_heads %d, max_seq %d, t %d)", c->batch,
                 c->kv_heads, c->max_seq, t);
+  if (c->max_seq > (1 << 24)) return fail(MQ_ERR_INVALID_ARG, "max_seq %d exceeds 2^24", c->max_seq);
   if (c->head_dim != 64 && c->head_dim != 128)
     return fail(MQ_ERR_INVALID_ARG, "head_dim %d is not 64 or 128", c->head_dim);
   const int g = c->group_size;
@@ -784,7 +785,7 @@ static int check_attend(const mq_kv4_cache* c, int t, int q_heads, int max_len) 
     return fail(MQ_ERR_INVALID_ARG, "q_heads %d is not a multiple of kv_heads %d", q_heads, c->kv_heads);
   if (max_len < 1 || max_len > c->max_seq)
     return fail(MQ_ERR_INVALID_ARG, "max_len %d outside [1, max_seq=%d]", max_len, c->max_seq);
-  if ((long long)t * q_heads > (1 << 24) || (long long)c->batch * t * q_heads > (1ll << 28))
+  if ((long long)t * q_heads > (1 << 24) || (long long)c->batch * t * q_heads > (1ll << 24))
     return fail(MQ_ERR_INVALID_ARG, "too many query rows (batch %d, t %d, q_heads %d)", c->batch, t, q_heads);
   return MQ_OK;
 }

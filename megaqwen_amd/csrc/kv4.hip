@@ -3,7 +3,10 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "mq_device.h"
+#include "mq_nibble.h"
 #include "mq_q4.h"
 
 namespace {
@@ -82,34 +85,320 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(MqKv4 c, void* k, void* v
   }
 }
 
-// One wave per (sequence, query row, query head): lanes hold 2 (D = 128) or 1 values of the head.
-__global__ void __launch_bounds__(64)
-kv4_attend_kernel(MqKv4 c, const uint16_t* q, MqStrides qs, uint16_t* out, int Hq, int max_len,
-                  bool f16, float scale_log2) {
-  const int lane = threadIdx.x, h = blockIdx.x % Hq, t = blockIdx.x / Hq, b = blockIdx.y;
-  const int hk = h / (Hq / c.Hkv), ng = c.D / c.G, per = c.D / 64;
-  const long long end = min((long long)c.lengths[b] - c.T + t + 1, (long long)min(c.S, max_len));
-  float qv[2] = {0.f, 0.f}, o[2] = {0.f, 0.f}, m = -INFINITY, l = 0.f;
-  for (int e = 0; e < per; ++e) qv[e] = from16(q[b * qs.b + t * qs.t + h * qs.h + per * lane + e], f16);
-  for (long long p = 0; p < end; ++p) {
-    const size_t row = ((size_t)b * c.Hkv + hk) * c.S + p;
-    const int g = per * lane / c.G;
-    float s = 0.f, vv[2];
-    for (int e = 0; e < per; ++e) {
-      const int d = per * lane + e;
-      const int ku = (c.kq[row * (c.D / 2) + d / 2] >> (4 * (d & 1))) & 15;
-      const int vu = (c.vq[row * (c.D / 2) + d / 2] >> (4 * (d & 1))) & 15;
-      s = fmaf(qv[e], bf16_to_f32(c.scales[(row * 2) * ng + g]) * (float)(ku - 8), s);
-      vv[e] = bf16_to_f32(c.scales[(row * 2 + 1) * ng + g]) * (float)(vu - 8);
+// ---- attention
+//
+// A workgroup is (sequence, kv head, a tile of its query rows, a range of positions); its 4 waves take
+// 32 positions at a time and join their (max, sum, O) at the end.  Query rows of a kv head are
+// r = t (Hq / Hkv) + head, so that a cached row is read once for all of them.
+//   * S = K Q^T by 16 x 16 x 32 products of the codes (mq_nibble.h) and the unrounded queries.  A
+//     key row has a scale per group of its dims, which no product can sum over: the 16 columns are
+//     (query row, group) pairs, column c holding row c / NG with all dims outside group c % NG
+//     zero.  Each score is the sum of its NG columns, times their scales, over neighbouring lanes.
+//   * the result's layout, a lane with 2 x 4 positions of one column, is the operand layout of
+//     O^T += V^T P^T: the weights go from registers into the next product.  Column (row, g) carries
+//     the weights times the value scales of group g, and only the dims of group g are kept of it.
+//   * weights enter as a truncated bf16 and the bf16 of the remainder (16 bits of each), so that their
+//     rounding stays far below the output's; one bf16 would add an error of the output's own size.
+// Softmax statistics and sums are fp32.  Codes are 4 bytes (8 dims) per lane for values, so that a
+// lane sees 8 positions of the same dims without a transpose through LDS.
+#define AT_WAVES 4
+#define AT_TILE 32                 // positions per wave and step
+#define AT_RAISE 8.0f              // a column's reference point moves when a score exceeds it by 2^8
+#define AT_BIAS (NB_OFFSET + 8.0f)
+
+struct AtArgs {
+  MqKv4 c;
+  const uint16_t* q;
+  MqStrides qs;
+  uint16_t* out;
+  float2* ml;                      // [rows][nsplit] (max, sum) and
+  float* part;                     // [rows][nsplit][D] unnormalised sums, if nsplit > 1
+  int Hq, ratio, max_len, nsplit, row_tiles;
+  float scale_log2;
+};
+
+template <bool F16, int D, int NG, int CT>
+__global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) {
+  constexpr int KW = D / 32;       // words of a key row per lane: dims (D / 4) j + 8 s + ..
+  constexpr int DPL = D / 16;      // dims of a value row per lane
+  constexpr int RQ = 16 / NG;      // query rows per column tile
+  constexpr int G = D / NG;
+  __shared__ float red[AT_WAVES][4 * DPL][64];
+  __shared__ float2 red_ml[AT_WAVES][CT][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, j = lane >> 4, g = col % NG;
+  // the kv head is the fastest index: workgroups go round the 8 XCDs, so that those that read the
+  // same rows share an L2
+  int id = blockIdx.x;
+  const int hk = id % a.c.Hkv; id /= a.c.Hkv;
+  const int rt = id % a.row_tiles; id /= a.row_tiles;
+  const int split = id % a.nsplit, b = id / a.nsplit;
+  const int rows = a.c.T * a.ratio, r0 = rt * (CT * RQ);
+  const int cap = min(a.c.S, a.max_len);
+  const long long first = (long long)a.c.lengths[b] - a.c.T + 1;      // positions of query t: first + t
+  auto limit = [&](int r) { return (int)max(0ll, min((long long)cap, first + r / a.ratio)); };
+  const int end = limit(min(r0 + CT * RQ, rows) - 1), sure = limit(r0);
+  const int chunk = ((end + a.nsplit - 1) / a.nsplit + AT_TILE - 1) / AT_TILE * AT_TILE;
+  const int p0 = split * chunk, p1 = min(end, p0 + chunk);
+
+  uint4 qf[CT][KW];
+  float cinit[CT], m[CT], l[CT], sv[CT];
+  int lim[CT];
+  nb_f32x4 acc[CT][DPL];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int r = r0 + ct * RQ + col / NG;
+    const bool there = r < rows;
+    const int t = there ? r / a.ratio : 0, h = there ? hk * a.ratio + r % a.ratio : 0;
+    const uint16_t* qr = a.q + b * a.qs.b + t * a.qs.t + h * a.qs.h;
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < KW; ++s) {
+      const int d = (D / 4) * j + 8 * s;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (there && d / G == g) x = nb_order8(nb_load16(qr + d));
+      qf[ct][s] = x;
+      sum += nb_sum8<F16>(x);
     }
-    s = wave_sum(s) * scale_log2;
-    const float mn = fmaxf(m, s), alpha = exp2f(m - mn), w = exp2f(s - mn);
-    m = mn;
-    l = fmaf(l, alpha, w);
-    for (int e = 0; e < per; ++e) o[e] = fmaf(o[e], alpha, w * vv[e]);
+    cinit[ct] = -AT_BIAS * sum_xor32(sum_xor16(sum));
+    lim[ct] = there ? limit(r) : 0;
+    m[ct] = -INFINITY;
+    l[ct] = sv[ct] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[ct][i] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  uint16_t* dst = out + (((size_t)b * c.T + t) * Hq + h) * c.D + per * lane;
-  for (int e = 0; e < per; ++e) dst[e] = to16(end > 0 ? o[e] / l : 0.f, f16);
+
+  // rows of this (sequence, kv head): loads beyond its last row in sight return 0 without an access
+  const size_t row = ((size_t)b * a.c.Hkv + hk) * a.c.S;
+  auto rsrc = [&](const void* base, int row_bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + row * row_bytes), (short)0, end * row_bytes, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t kr = rsrc(a.c.kq, D / 2), vr = rsrc(a.c.vq, D / 2), sr = rsrc(a.c.scales, 4 * NG);
+  struct Tile {
+    uint32_t k[2][KW], v[8], ks[8], vs[8];
+  };
+  auto load = [&](Tile& x, int p) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int ko = (p + 16 * t + col) * (D / 2) + j * (4 * KW);
+      if constexpr (KW == 4) {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b128(kr, ko, 0, 0);
+        for (int s = 0; s < 4; ++s) x.k[t][s] = w[s];
+      } else {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(kr, ko, 0, 0);
+        for (int s = 0; s < 2; ++s) x.k[t][s] = w[s];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int pos = p + 16 * t + 4 * j + i, e = 4 * t + i;
+        if constexpr (DPL == 8) x.v[e] = __builtin_amdgcn_raw_buffer_load_b32(vr, pos * (D / 2) + 4 * col, 0, 0);
+        else x.v[e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vr, pos * (D / 2) + 2 * col, 0, 0);
+        if constexpr (NG == 1) {
+          const uint32_t w = __builtin_amdgcn_raw_buffer_load_b32(sr, pos * 4, 0, 0);
+          x.ks[e] = w << 16;
+          x.vs[e] = w & 0xffff0000u;
+        } else {
+          x.ks[e] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * (4 * NG) + 2 * g, 0, 0) << 16;
+          x.vs[e] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * (4 * NG) + 2 * NG + 2 * g, 0, 0) << 16;
+        }
+      }
+    }
+  };
+
+  auto step = [&](const Tile& x, int p) {
+    // scores z[ct][e] (log2 units) of positions p + 16 (e / 4) + 4 j + e % 4
+    float z[CT][8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      nb_f32x4 s[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[ct] = nb_f32x4{cinit[ct], cinit[ct], cinit[ct], cinit[ct]};
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const uint4 kx = nb_expand8<F16>(x.k[t][w]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[ct] = nb_mfma<F16>(kx, qf[ct][w], s[ct]);
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = s[ct][i] * __uint_as_float(x.ks[4 * t + i]);
+          if constexpr (NG >= 2) v += dpp_f<MQ_DPP_QUAD_XOR1>(v);
+          if constexpr (NG >= 4) v += dpp_f<MQ_DPP_QUAD_XOR2>(v);
+          z[ct][4 * t + i] = v * a.scale_log2;
+        }
+    }
+    if (p + AT_TILE > sure) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (p + 16 * (e >> 2) + 4 * j + (e & 3) >= lim[ct]) z[ct][e] = -INFINITY;
+    }
+    uint4 ph[CT], pl[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float mt = fmaxf(fmaxf(fmaxf(z[ct][0], z[ct][1]), fmaxf(z[ct][2], z[ct][3])),
+                       fmaxf(fmaxf(z[ct][4], z[ct][5]), fmaxf(z[ct][6], z[ct][7])));
+      mt = max_xor32(max_xor16(mt));
+      if (__builtin_amdgcn_ballot_w64(mt > m[ct] + AT_RAISE) != 0) {
+        const bool up = mt > m[ct] + AT_RAISE;
+        const float alpha = up ? __builtin_amdgcn_exp2f(m[ct] - mt) : 1.0f;
+        m[ct] = up ? mt : m[ct];
+        l[ct] *= alpha;
+        sv[ct] *= alpha;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) acc[ct][i] *= alpha;
+      }
+      // (nothing seen yet: every weight of the column is 2^-inf)
+      const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        float w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float p_ = __builtin_amdgcn_exp2f(z[ct][e + i] - ref);
+          l[ct] += p_;
+          // a masked position's scale may be anything
+          w[i] = z[ct][e + i] == -INFINITY ? 0.f : p_ * __uint_as_float(x.vs[e + i]);
+          sv[ct] += w[i];
+        }
+        hi[e / 2] = __builtin_amdgcn_perm(__float_as_uint(w[1]), __float_as_uint(w[0]), 0x07060302u);
+        lo[e / 2] = (uint32_t)f32_to_bf16(w[0] - __uint_as_float(__float_as_uint(w[0]) & 0xffff0000u)) |
+                    ((uint32_t)f32_to_bf16(w[1] - __uint_as_float(__float_as_uint(w[1]) & 0xffff0000u)) << 16);
+      }
+      ph[ct] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      pl[ct] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    // value codes of position pairs in the halves of a word: words f of wl hold dims DPL col + f
+    uint32_t wl[4], wh[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      wl[t] = __builtin_amdgcn_perm(x.v[2 * t + 1], x.v[2 * t], 0x05040100u);
+      if constexpr (DPL == 8) wh[t] = __builtin_amdgcn_perm(x.v[2 * t + 1], x.v[2 * t], 0x07060302u);
+    }
+    auto values = [&](auto f_tag, const uint32_t (&w)[4], int i) {
+      constexpr int f = decltype(f_tag)::value;
+      const uint4 va = make_uint4(nb_pair<false, f>(w[0]), nb_pair<false, f>(w[1]), nb_pair<false, f>(w[2]), nb_pair<false, f>(w[3]));
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        acc[ct][i] = nb_mfma<false>(va, ph[ct], acc[ct][i]);
+        acc[ct][i] = nb_mfma<false>(va, pl[ct], acc[ct][i]);
+      }
+    };
+    values(std::integral_constant<int, 0>(), wl, 0);
+    values(std::integral_constant<int, 1>(), wl, 1);
+    values(std::integral_constant<int, 2>(), wl, 2);
+    values(std::integral_constant<int, 3>(), wl, 3);
+    if constexpr (DPL == 8) {
+      values(std::integral_constant<int, 0>(), wh, 4);
+      values(std::integral_constant<int, 1>(), wh, 5);
+      values(std::integral_constant<int, 2>(), wh, 6);
+      values(std::integral_constant<int, 3>(), wh, 7);
+    }
+  };
+
+  int p = p0 + AT_TILE * wave;
+  if (p < p1) {
+    Tile x;
+    load(x, p);
+    for (; p < p1; p += AT_TILE * AT_WAVES) {
+      Tile y;
+      load(y, p + AT_TILE * AT_WAVES);       // (past the end: zeros, not used)
+      step(x, p);
+      x = y;
+    }
+  }
+
+  // Join the waves.  A column's O, without the codes' offset, is in value order i' DPL + i, where
+  // dim = DPL (4 j + i') + i.
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    l[ct] = sum_xor32(sum_xor16(l[ct]));
+    sv[ct] = sum_xor32(sum_xor16(sv[ct]));
+    if (j == 0) red_ml[wave][ct][col] = make_float2(m[ct], l[ct]);
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < DPL; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[wave][e * DPL + i][lane] = fmaf(-AT_BIAS, sv[ct], acc[ct][i][e]);
+    __syncthreads();
+    float mx = -INFINITY, sum = 0.f, f[AT_WAVES];
+#pragma unroll
+    for (int w = 0; w < AT_WAVES; ++w) mx = fmaxf(mx, red_ml[w][ct][col].x);
+#pragma unroll
+    for (int w = 0; w < AT_WAVES; ++w) {
+      const float2 v = red_ml[w][ct][col];
+      f[w] = v.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v.x - mx);
+      sum = fmaf(v.y, f[w], sum);
+    }
+    // wave i' of the workgroup: dims DPL (4 j + i') .. + DPL of the lane's column
+    float o[DPL];
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) {
+      o[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < AT_WAVES; ++w) o[i] = f[w] == 0.f ? o[i] : fmaf(red[w][wave * DPL + i][lane], f[w], o[i]);
+    }
+    const int r = r0 + ct * RQ + col / NG, d = DPL * (4 * j + wave);
+    if (r >= rows || d / G != g) continue;
+    const size_t at = ((size_t)b * a.c.T + r / a.ratio) * a.Hq + hk * a.ratio + r % a.ratio;
+    if (a.nsplit == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      uint32_t w[DPL / 2];
+#pragma unroll
+      for (int i = 0; i < DPL; i += 2)
+        w[i / 2] = (uint32_t)to16(o[i] * inv, F16) | ((uint32_t)to16(o[i + 1] * inv, F16) << 16);
+      uint32_t* dst = (uint32_t*)(a.out + at * D + d);
+#pragma unroll
+      for (int i = 0; i < DPL / 2; ++i) dst[i] = w[i];
+    } else {
+      if (d == 0) a.ml[at * a.nsplit + split] = make_float2(mx, sum);
+      if (sum != 0.f) {
+        float* dst = a.part + (at * a.nsplit + split) * D + d;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) dst[i] = o[i];
+      }
+    }
+  }
+}
+
+// Joins the ranges of a query row: one workgroup of D threads per row.
+template <int D>
+__global__ void __launch_bounds__(D) kv4_join_kernel(const float2* ml, const float* part, uint16_t* out, int nsplit, bool f16) {
+  const size_t at = blockIdx.x;
+  const float2* mr = ml + at * nsplit;
+  float mx = -INFINITY, sum = 0.f, o = 0.f;
+  for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, mr[s].x);
+  for (int s = 0; s < nsplit; ++s) {
+    const float2 v = mr[s];
+    if (v.y == 0.f) continue;                 // no position of this range: nothing was stored
+    const float f = __builtin_amdgcn_exp2f(v.x - mx);
+    sum = fmaf(v.y, f, sum);
+    o = fmaf(part[(at * nsplit + s) * D + threadIdx.x], f, o);
+  }
+  out[at * D + threadIdx.x] = to16(sum == 0.f ? 0.f : o / sum, f16);
+}
+
+// How a call is laid out: column tiles per workgroup and ranges of positions.
+struct AtPlan {
+  int ct, row_tiles, nsplit;
+};
+AtPlan at_plan(int B, int T, int Hq, int Hkv, int D, int G, int max_len) {
+  AtPlan p;
+  const int rq = 16 / (D / G), rows = T * (Hq / Hkv);
+  p.ct = rows <= rq ? 1 : 2;
+  p.row_tiles = (rows + p.ct * rq - 1) / (p.ct * rq);
+  const long long wgs = (long long)B * Hkv * p.row_tiles;
+  const int most = max_len <= 512 ? 1 : (max_len + 255) / 256;
+  const long long want = (512 + wgs - 1) / wgs;
+  p.nsplit = (int)(want < most ? want : most);
+  return p;
 }
 
 int launched() { return hipGetLastError() == hipSuccess ? 0 : -1; }
@@ -131,11 +420,41 @@ int mq_launch_kv4_read(const MqKv4& c, void* k, void* v, int o_type, hipStream_t
   return launched();
 }
 
-size_t mq_kv4_attend_workspace(int, int, int, int, int, int, int) { return 0; }
+size_t mq_kv4_attend_workspace(int B, int T, int Hq, int Hkv, int D, int G, int max_len) {
+  const AtPlan p = at_plan(B, T, Hq, Hkv, D, G, max_len);
+  if (p.nsplit == 1) return 0;
+  const size_t rows = (size_t)B * T * Hq * p.nsplit;
+  return (rows * sizeof(float2) + 15) / 16 * 16 + rows * D * sizeof(float);
+}
 
 int mq_launch_kv4_attend(const MqKv4& c, const uint16_t* q, MqStrides qs, uint16_t* out, int Hq,
-                         int max_len, bool f16, float scale_log2, void*, hipStream_t stream) {
-  hipLaunchKernelGGL(kv4_attend_kernel, dim3((unsigned)(c.T * Hq), c.B), dim3(64), 0, stream, c, q, qs,
-                     out, Hq, max_len, f16, scale_log2);
+                         int max_len, bool f16, float scale_log2, void* ws, hipStream_t stream) {
+  const AtPlan p = at_plan(c.B, c.T, Hq, c.Hkv, c.D, c.G, max_len);
+  const size_t rows = (size_t)c.B * c.T * Hq;
+  AtArgs a = {c, q, qs, out, (float2*)ws, (float*)((char*)ws + (rows * p.nsplit * sizeof(float2) + 15) / 16 * 16),
+              Hq, Hq / c.Hkv, max_len, p.nsplit, p.row_tiles, scale_log2};
+  const dim3 grid((unsigned)((long long)c.B * c.Hkv * p.row_tiles * p.nsplit)), block(64 * AT_WAVES);
+  auto go = [&](auto f16_, auto d, auto ng) {
+    constexpr bool F = decltype(f16_)::value;
+    constexpr int D = decltype(d)::value, NG = decltype(ng)::value;
+    if (p.ct == 1) hipLaunchKernelGGL((kv4_attend_kernel<F, D, NG, 1>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((kv4_attend_kernel<F, D, NG, 2>), grid, block, 0, stream, a);
+    if (p.nsplit > 1)
+      hipLaunchKernelGGL((kv4_join_kernel<D>), dim3((unsigned)rows), dim3(D), 0, stream, a.ml, a.part, out, p.nsplit, F);
+  };
+  auto pick = [&](auto f16_) {
+    using std::integral_constant;
+    const int ng = c.D / c.G;
+    if (c.D == 128) {
+      if (ng == 4) go(f16_, integral_constant<int, 128>(), integral_constant<int, 4>());
+      else if (ng == 2) go(f16_, integral_constant<int, 128>(), integral_constant<int, 2>());
+      else go(f16_, integral_constant<int, 128>(), integral_constant<int, 1>());
+    } else {
+      if (ng == 2) go(f16_, integral_constant<int, 64>(), integral_constant<int, 2>());
+      else go(f16_, integral_constant<int, 64>(), integral_constant<int, 1>());
+    }
+  };
+  if (f16) pick(std::true_type());
+  else pick(std::false_type());
   return launched();
 }
