@@ -684,7 +684,7 @@ static int launch_result(int rc) {
 int mq_w4_linear(const void* d_x, const void* d_qweight, const void* d_scales, const void* d_zeros,
                  const void* d_residual, void* d_out, int rows, int n, int k, int group_size,
                  int x_dtype, int scale_dtype, int out_dtype, void* stream) {
-  if (rows < 0 || n < 0 || k < 1)
+  if (rows < 0 || n < 0 || k < 1 || k > (1 << 24))
     return fail(MQ_ERR_INVALID_ARG, "bad size (rows %d, n %d, k %d)", rows, n, k);
   if (group_size != 32 && group_size != 64 && group_size != 128)
     return fail(MQ_ERR_INVALID_ARG, "group_size %d is not 32, 64 or 128", group_size);
