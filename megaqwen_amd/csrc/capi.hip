@@ -684,7 +684,7 @@ static int launch_result(int rc) {
 int mq_w4_linear(const void* d_x, const void* d_qweight, const void* d_scales, const void* d_zeros,
                  const void* d_residual, void* d_out, int rows, int n, int k, int group_size,
                  int x_dtype, int scale_dtype, int out_dtype, void* stream) {
-  if (rows < 0 || n < 0 || k < 1 || k > (1 << 24))
+  if (rows < 0 || n < 0 || k < 1 || k > (1 << 22))
     return fail(MQ_ERR_INVALID_ARG, "bad size (rows %d, n %d, k %d)", rows, n, k);
   if (group_size != 32 && group_size != 64 && group_size != 128)
     return fail(MQ_ERR_INVALID_ARG, "group_size %d is not 32, 64 or 128", group_size);
@@ -725,7 +725,7 @@ static int check_kv4(const mq_kv4_cache* c, const int32_t* d_lengths, int t, MqK
   const int g = c->group_size;
   if ((g != 32 && g != 64 && g != 128) || g > c->head_dim)
     return fail(MQ_ERR_INVALID_ARG, "group_size %d is not 32, 64 or 128, at most head_dim", g);
-  if (c->batch > 65535 || (long long)c->batch * t * c->kv_heads > (1ll << 28))
+  if (c->batch > 65535 || (long long)t * c->kv_heads > (1 << 26))
     return fail(MQ_ERR_INVALID_ARG, "too many rows (batch %d, t %d, kv_heads %d)", c->batch, t, c->kv_heads);
   if (c->batch == 0 || t == 0) return MQ_OK;
   if (c->k_codes == nullptr || c->v_codes == nullptr || c->scales == nullptr || d_lengths == nullptr)

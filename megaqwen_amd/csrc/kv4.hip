@@ -11,77 +11,81 @@
 
 namespace {
 
-MQ_DEV float from16(uint32_t bits, bool f16) {
-  return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)bits) : bf16_to_f32((bf16_t)bits);
-}
 MQ_DEV uint16_t to16(float v, bool f16) {
   return f16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : f32_to_bf16(v);
 }
 
-// One thread per group of G values of a key (i = 0) or value (i = 1) row.
-//   s = bf16(max|x| / 7), u = clamp(rint(x / s), -7, 7) + 8; s = 0: u = 8; a group that holds an
-//   infinity or a NaN gets s = NaN, so that all of its values read as NaN.
-__global__ void __launch_bounds__(256)
-kv4_append_kernel(MqKv4 c, const uint16_t* k, MqStrides ks, const uint16_t* v, MqStrides vs, bool f16) {
-  const int ng = c.D / c.G;
-  long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= (long long)c.B * c.T * c.Hkv * 2 * ng) return;
-  const int g = (int)(id % ng); id /= ng;
-  const int which = (int)(id & 1); id >>= 1;
-  const int h = (int)(id % c.Hkv); id /= c.Hkv;
-  const int t = (int)(id % c.T), b = (int)(id / c.T);
-  const long long pos = (long long)c.lengths[b] - c.T + t;
-  if (pos < 0 || pos >= c.S) return;
+// One thread per 8 values of a key (which = 0) or value row, neighbours along the row:
+//   s = bf16(max|x| / 7) over the group's G / 8 threads, u = clamp(rint(x / s), -7, 7) + 8; s = 0:
+//   u = 8; a group that holds an infinity or a NaN gets s = NaN, so that all of its values read as NaN.
+// The quotient is the correctly rounded fp32 one: a bf16 or fp16 value over a bf16 scale is never so
+// close to half a step that this could round to the other side of it.
+template <bool F16, int G>
+__global__ void __launch_bounds__(256) kv4_append_kernel(MqKv4 c, const uint16_t* k, MqStrides ks, const uint16_t* v, MqStrides vs) {
+  const unsigned per = c.D / 8, n = (unsigned)c.T * c.Hkv * per, id = blockIdx.x * 256 + threadIdx.x;
+  const int b = blockIdx.y;
+  if (id >= 2 * n) return;
+  const bool which = id >= n;
+  const unsigned at = which ? id - n : id, piece = at % per, row_id = at / per;
+  const int h = row_id % c.Hkv, t = row_id / c.Hkv;
   const MqStrides st = which ? vs : ks;
-  const uint16_t* x = (which ? v : k) + b * st.b + t * st.t + h * st.h + g * c.G;
-  float amax = 0.f;
-  bool bad = false;
-  for (int i = 0; i < c.G; ++i) {
-    const float f = fabsf(from16(x[i], f16));
-    bad |= !(f < INFINITY);
-    amax = fmaxf(amax, f);
-  }
-  const uint16_t sb = bad ? 0x7fc0 : f32_to_bf16(amax / 7.0f);
+  const uint4 x = nb_load16((which ? v : k) + b * st.b + t * st.t + h * st.h + 8 * piece);
+  const long long pos = (long long)c.lengths[b] - c.T + t;
+  const float f[8] = {nb_lo<F16>(x.x), nb_hi<F16>(x.x), nb_lo<F16>(x.y), nb_hi<F16>(x.y),
+                      nb_lo<F16>(x.z), nb_hi<F16>(x.z), nb_lo<F16>(x.w), nb_hi<F16>(x.w)};
+  // (maximum keeps a NaN; the lanes of a group are in the same row of 16)
+  float m = fabsf(f[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = __builtin_elementwise_maximum(m, fabsf(f[i]));
+  m = __builtin_elementwise_maximum(m, dpp_f<MQ_DPP_QUAD_XOR1>(m));
+  m = __builtin_elementwise_maximum(m, dpp_f<MQ_DPP_QUAD_XOR2>(m));
+  if constexpr (G >= 64) m = __builtin_elementwise_maximum(m, dpp_f<MQ_DPP_ROW_HALF_MIRROR>(m));
+  if constexpr (G >= 128) m = __builtin_elementwise_maximum(m, dpp_f<MQ_DPP_ROW_MIRROR>(m));
+  const uint16_t sb = m < INFINITY ? f32_to_bf16(m / 7.0f) : 0x7fc0;
   const float s = bf16_to_f32(sb);
-  const size_t row = ((size_t)b * c.Hkv + h) * c.S + pos;
-  c.scales[(row * 2 + which) * ng + g] = sb;
-  uint8_t* dst = (which ? c.vq : c.kq) + row * (c.D / 2) + g * (c.G / 2);
-  for (int i = 0; i < c.G; i += 2) {
-    uint32_t u[2];
-    for (int e = 0; e < 2; ++e) {
-      const float r = s > 0.f ? rintf(from16(x[i + e], f16) / s) : 0.f;
-      u[e] = (uint32_t)(int)(fminf(fmaxf(r, -7.f), 7.f) + 8.f);
-    }
-    dst[i / 2] = (uint8_t)(u[0] | (u[1] << 4));
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float r = s > 0.f ? rintf(f[i] / s) : 0.f;
+    w |= (uint32_t)(int)(fminf(fmaxf(r, -7.f), 7.f) + 8.f) << (4 * i);
   }
+  if (pos < 0 || pos >= c.S) return;
+  const size_t row = ((size_t)b * c.Hkv + h) * c.S + pos;
+  ((uint32_t*)(which ? c.vq : c.kq))[row * per + piece] = w;
+  if (piece % (G / 8) == 0) c.scales[(row * 2 + which) * (c.D / G) + piece / (G / 8)] = sb;
 }
 
-// One thread per byte (two values) of a row; rows outside [0, S) read as 0.
+// One thread per 8 values; rows outside [0, S) read as 0.
 __global__ void __launch_bounds__(256) kv4_read_kernel(MqKv4 c, void* k, void* v, int o_type) {
-  const int half = c.D / 2, ng = c.D / c.G;
-  long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= (long long)c.B * c.T * c.Hkv * 2 * half) return;
-  const int d = (int)(id % half); id /= half;
-  const int which = (int)(id & 1); id >>= 1;
-  const size_t o = (size_t)id * c.D + 2 * d;
-  const int h = (int)(id % c.Hkv); id /= c.Hkv;
-  const int t = (int)(id % c.T), b = (int)(id / c.T);
+  const unsigned per = c.D / 8, n = (unsigned)c.T * c.Hkv * per, id = blockIdx.x * 256 + threadIdx.x;
+  const int b = blockIdx.y;
+  if (id >= 2 * n) return;
+  const bool which = id >= n;
+  const unsigned at = which ? id - n : id, piece = at % per, row_id = at / per;
+  const int h = row_id % c.Hkv, t = row_id / c.Hkv;
   const long long pos = (long long)c.lengths[b] - c.T + t;
-  float lo = 0.f, hi = 0.f;
+  float s = 0.f;
+  uint32_t u = 0;
   if (pos >= 0 && pos < c.S) {
     const size_t row = ((size_t)b * c.Hkv + h) * c.S + pos;
-    const float s = bf16_to_f32(c.scales[(row * 2 + which) * ng + 2 * d / c.G]);
-    const uint32_t u = (which ? c.vq : c.kq)[row * half + d];
-    lo = s * (float)((int)(u & 15) - 8);
-    hi = s * (float)((int)(u >> 4) - 8);
+    s = bf16_to_f32(c.scales[(row * 2 + which) * (c.D / c.G) + 8 * piece / c.G]);
+    u = ((const uint32_t*)(which ? c.vq : c.kq))[row * per + piece];
   }
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = s * (float)((int)((u >> (4 * i)) & 15u) - 8);
+  const size_t o = ((size_t)b * n + at) * 8;
   void* out = which ? v : k;
   if (o_type == MQ_T_F32) {
-    ((float*)out)[o] = lo;
-    ((float*)out)[o + 1] = hi;
+    float4* dst = (float4*)((float*)out + o);
+    dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+    dst[1] = make_float4(f[4], f[5], f[6], f[7]);
   } else {
-    ((uint16_t*)out)[o] = to16(lo, o_type == MQ_T_F16);
-    ((uint16_t*)out)[o + 1] = to16(hi, o_type == MQ_T_F16);
+    const bool f16 = o_type == MQ_T_F16;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)to16(f[2 * i], f16) | ((uint32_t)to16(f[2 * i + 1], f16) << 16);
+    *(uint4*)((uint16_t*)out + o) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -368,21 +372,56 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
   }
 }
 
-// Joins the ranges of a query row: one workgroup of D threads per row.
-template <int D>
-__global__ void __launch_bounds__(D) kv4_join_kernel(const float2* ml, const float* part, uint16_t* out, int nsplit, bool f16) {
-  const size_t at = blockIdx.x;
+// Joins the ranges of a query row.  A row is WAVES waves (1 for few ranges, 4 for many), a thread 4
+// dims of every SLOTS-th range; ranges without a position (sum 0) have nothing stored.
+template <int D, int WAVES>
+__global__ void __launch_bounds__(256) kv4_join_kernel(const float2* ml, const float* part, uint16_t* out, int rows, int nsplit, bool f16) {
+  constexpr int DT = D / 4, SLOTS = 64 * WAVES / DT;
+  __shared__ float4 red[4][DT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = lane % DT, slot = (threadIdx.x & (64 * WAVES - 1)) / DT;
+  const size_t at = (size_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
+  if (at >= (size_t)rows) return;                       // (whole waves; with 4 waves a row there is no rest)
   const float2* mr = ml + at * nsplit;
-  float mx = -INFINITY, sum = 0.f, o = 0.f;
-  for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, mr[s].x);
-  for (int s = 0; s < nsplit; ++s) {
+  float mx = -INFINITY, sum = 0.f;
+  for (int s = lane; s < nsplit; s += 64) mx = fmaxf(mx, mr[s].x);
+  mx = wave_max(mx);
+  for (int s = lane; s < nsplit; s += 64) {
     const float2 v = mr[s];
-    if (v.y == 0.f) continue;                 // no position of this range: nothing was stored
-    const float f = __builtin_amdgcn_exp2f(v.x - mx);
-    sum = fmaf(v.y, f, sum);
-    o = fmaf(part[(at * nsplit + s) * D + threadIdx.x], f, o);
+    sum = v.y == 0.f ? sum : fmaf(v.y, __builtin_amdgcn_exp2f(v.x - mx), sum);
   }
-  out[at * D + threadIdx.x] = to16(sum == 0.f ? 0.f : o / sum, f16);
+  sum = wave_sum(sum);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = slot; s < nsplit; s += SLOTS) {
+    const float4 p = ((const float4*)part)[(at * nsplit + s) * DT + d];
+    const float2 v = mr[s];
+    const float f = __builtin_amdgcn_exp2f(v.x - mx);
+    o.x = v.y == 0.f ? o.x : fmaf(p.x, f, o.x);
+    o.y = v.y == 0.f ? o.y : fmaf(p.y, f, o.y);
+    o.z = v.y == 0.f ? o.z : fmaf(p.z, f, o.z);
+    o.w = v.y == 0.f ? o.w : fmaf(p.w, f, o.w);
+  }
+  auto across = [](float v) {
+    v = sum_xor32(v);
+    return DT == 16 ? sum_xor16(v) : v;
+  };
+  o = make_float4(across(o.x), across(o.y), across(o.z), across(o.w));
+  if constexpr (WAVES == 4) {
+    if (lane < DT) red[wave][lane] = o;
+    __syncthreads();
+    if (threadIdx.x >= DT) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 p = red[w][d];
+      o = make_float4(o.x + p.x, o.y + p.y, o.z + p.z, o.w + p.w);
+    }
+  } else if (lane >= DT) {
+    return;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const uint32_t lo = (uint32_t)to16(o.x * inv, f16) | ((uint32_t)to16(o.y * inv, f16) << 16);
+  const uint32_t hi = (uint32_t)to16(o.z * inv, f16) | ((uint32_t)to16(o.w * inv, f16) << 16);
+  ((uint2*)out)[at * DT + d] = make_uint2(lo, hi);
 }
 
 // How a call is laid out: column tiles per workgroup and ranges of positions.
@@ -405,18 +444,30 @@ int launched() { return hipGetLastError() == hipSuccess ? 0 : -1; }
 
 }  // namespace
 
+// (8 values per thread; the host has checked T Hkv <= 2^26)
+static dim3 kv4_row_grid(const MqKv4& c) {
+  const unsigned n = 2u * (unsigned)c.T * c.Hkv * (c.D / 8);
+  return dim3((n + 255) / 256, c.B);
+}
+
 int mq_launch_kv4_append(const MqKv4& c, const uint16_t* k, MqStrides ks, const uint16_t* v,
                          MqStrides vs, bool f16, hipStream_t stream) {
-  const long long n = (long long)c.B * c.T * c.Hkv * 2 * (c.D / c.G);
-  hipLaunchKernelGGL(kv4_append_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, c, k,
-                     ks, v, vs, f16);
+  auto go = [&](auto f16_, auto g) {
+    hipLaunchKernelGGL((kv4_append_kernel<decltype(f16_)::value, decltype(g)::value>), kv4_row_grid(c), dim3(256), 0, stream, c,
+                       k, ks, v, vs);
+  };
+  auto pick = [&](auto f16_) {
+    if (c.G == 32) go(f16_, std::integral_constant<int, 32>());
+    else if (c.G == 64) go(f16_, std::integral_constant<int, 64>());
+    else go(f16_, std::integral_constant<int, 128>());
+  };
+  if (f16) pick(std::true_type());
+  else pick(std::false_type());
   return launched();
 }
 
 int mq_launch_kv4_read(const MqKv4& c, void* k, void* v, int o_type, hipStream_t stream) {
-  const long long n = (long long)c.B * c.T * c.Hkv * c.D;
-  hipLaunchKernelGGL(kv4_read_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, c, k, v,
-                     o_type);
+  hipLaunchKernelGGL(kv4_read_kernel, kv4_row_grid(c), dim3(256), 0, stream, c, k, v, o_type);
   return launched();
 }
 
@@ -439,8 +490,10 @@ int mq_launch_kv4_attend(const MqKv4& c, const uint16_t* q, MqStrides qs, uint16
     constexpr int D = decltype(d)::value, NG = decltype(ng)::value;
     if (p.ct == 1) hipLaunchKernelGGL((kv4_attend_kernel<F, D, NG, 1>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((kv4_attend_kernel<F, D, NG, 2>), grid, block, 0, stream, a);
-    if (p.nsplit > 1)
-      hipLaunchKernelGGL((kv4_join_kernel<D>), dim3((unsigned)rows), dim3(D), 0, stream, a.ml, a.part, out, p.nsplit, F);
+    if (p.nsplit >= 16)
+      hipLaunchKernelGGL((kv4_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a.ml, a.part, out, (int)rows, p.nsplit, F);
+    else if (p.nsplit > 1)
+      hipLaunchKernelGGL((kv4_join_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a.ml, a.part, out, (int)rows, p.nsplit, F);
   };
   auto pick = [&](auto f16_) {
     using std::integral_constant;

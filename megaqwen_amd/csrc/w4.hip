@@ -2,16 +2,25 @@
 //   out[m][n] = sum_g s[n][g] sum_{k in g} (u[n][k] - z[n][g]) x[m][k]  (+ residual[m][n])
 //
 // A wave takes 16 outputs n and up to 64 rows m, 128 inputs k at a time: lane (n = l % 16, j = l / 16)
-// loads the 16 bytes of codes 32 j .. 32 j + 31 of its output's row (64 bytes of 16 rows per load), which
-// become operands of 16 x 16 x 32 matrix products with a shift and an and-or per two codes
-// (mq_nibble.h); the matrix cores do the multiplying, so that one row costs what 16 do.  The rows of x
-// wait in LDS in operand order, with their sum over every group:
-//   sum_{k in g} (u - z) x = sum (16 + u) x - (16 + z) sum x,
-// the second term being where the products' sum starts.  It is scaled and added in fp32 per group.
+// loads the 16 bytes of codes 32 j .. 32 j + 31 of its output's row, which become operands of 16 x 16 x 32
+// matrix products with a shift and an and-or per two codes (mq_nibble.h): the matrix cores do the
+// multiplying, so that one row costs what 16 do.  A second product with the constant -(16 + z) takes the
+// offset and the zero point off,
+//   sum_{k in g} (u - z) x = sum (16 + u) x + sum -(16 + z) x,
+// both exact in fp32 but for the sums' roundings; matrix cycles are there to spare, vector instructions
+// are not.  A group's sum is scaled and added in fp32.
 // All four lanes of an output must work on the same group in one product.  With groups of 128 they do;
 // for 64 and 32 the words are first exchanged between the lanes of an output (permlane swaps, one
 // instruction per word or half of one), which keeps the 16-byte loads.
-// 8 waves share the rows of x: KW of them split the inputs of the same outputs and join at the end.
+//
+// Three kernels, by the sizes (w4_plan()):
+//   w4_direct_kernel   few outputs and up to 16 rows: the 8 waves of a workgroup split the inputs of 16
+//                      outputs and load their own pieces of x; nothing waits before the first product
+//   w4_whole_kernel    several tiles of 16 outputs per workgroup share the rows of x, which wait in LDS in
+//                      operand order; kw waves split a tile's inputs
+//   w4_stretch_kernel  the same where the rows do not fit: a stretch of inputs after the other, two in LDS
+// x through LDS also keeps the loads of weights ahead of their use: loads return in order, so one of x
+// behind them would wait for memory.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -26,9 +35,6 @@ namespace {
 #define W4_WAVES 8
 #define W4_THREADS (64 * W4_WAVES)
 #define W4_FAR 0x40000000               // a buffer offset behind every buffer: its load returns 0
-// blocks of 128 inputs that a wave has in flight, for mt tiles of 16 rows
-constexpr int w4_unroll(int mt) { return mt <= 2 ? 4 : 2; }
-#define W4_LDS 61440                    // bytes of x (and its sums) staged at a time
 
 MQ_DEV float w4_from16(uint32_t bits, bool f16) {
   return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)bits) : __uint_as_float(bits << 16);
@@ -40,6 +46,11 @@ MQ_DEV void w4_store(void* out, size_t i, float v, int type) {
 }
 MQ_DEV float w4_residual(const void* r, size_t i, int type) {
   return type == MQ_T_F32 ? ((const float*)r)[i] : w4_from16(((const uint16_t*)r)[i], type == MQ_T_F16);
+}
+MQ_DEV void w4_write(const MqW4Args& a, int m, int n, float v) {
+  const size_t at = (size_t)m * a.N + n;
+  if (a.residual != nullptr) v += w4_residual(a.residual, at, a.o_type);
+  w4_store(a.out, at, v, a.o_type);
 }
 
 // Words d[s] of lane j as step s of the products: afterwards step s's four lanes hold words of one group.
@@ -55,7 +66,13 @@ template <int G> MQ_DEV void w4_exchange(uint32_t (&d)[4]) {
     d[0] = p[0]; d[1] = p[1]; d[2] = q[0]; d[3] = q[1];
   }
 }
-// Where the 8 inputs 8 piece .. of a block of 128 are then: 4 * step + lane j
+// Step s of lane j is then on the 8 inputs 8 piece .. of the block,
+template <int G> MQ_DEV int w4_piece(int step, int j) {
+  if constexpr (G == 128) return 4 * j + step;
+  else if constexpr (G == 64) return 4 * ((j & 1) + 2 * (step >> 1)) + (step & 1) + 2 * (j >> 1);
+  else return 4 * step + j;
+}
+// and those inputs are at 4 * step + j.
 template <int G> MQ_DEV int w4_slot(int piece) {
   const int p = piece >> 2, d = piece & 3;         // loaded by lane p as word d
   if constexpr (G == 128) return 4 * d + p;
@@ -63,221 +80,419 @@ template <int G> MQ_DEV int w4_slot(int piece) {
   else return 4 * p + d;
 }
 
-struct W4Plan {
-  int blocks;         // of 128 inputs, the last one possibly cut
-  int kw;             // waves that split the inputs; W4_WAVES / kw tiles of 16 outputs per workgroup
-  int steps;          // times w4_unroll() blocks per wave for all of K
-  int chunk;          // such steps per staging of x
-  int lds;            // bytes
-  bool wide_scales;   // a block's scales (and zeros) are one aligned load
+// Scales and zero points of the NS groups of U blocks of 128 inputs of one output.
+template <int NS> struct W4Scales {
+  uint32_t s[(NS + 1) / 2], z[(NS + 3) / 4];
 };
-
-template <bool F16, int G, int MT, bool ONE>
-__global__ void __launch_bounds__(W4_THREADS, MT <= 2 ? 4 : 2) w4_kernel(MqW4Args a, W4Plan pl) {
-  constexpr int PER = 128 / G, U = w4_unroll(MT);      // groups of a block; blocks of a step
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = wave / pl.kw, kw = wave - nw * pl.kw;
-  const int n0 = (blockIdx.x * (W4_WAVES / pl.kw) + nw) * 16;
-  const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
-  const int groups = a.K / G, tile_rows = max(0, min(16, a.N - n0));
-  const int cblocks = pl.chunk * U * pl.kw;                  // blocks staged at a time
-  const int xstride = cblocks * 128 + 8;                             // (8: rows start in different banks)
-  uint16_t* xs = (uint16_t*)lds;                                     // [rows][block][step][j][8]
-  float* xsum = (float*)(lds + (((size_t)rows * xstride * 2 + 15) & ~(size_t)15));   // [group][16 MT]
-
-  // Rows of this wave's outputs: loads of rows >= N, and of inputs >= K, return 0 without an access.
-  auto rsrc = [&](const void* p, int row_bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)p + (size_t)n0 * row_bytes), (short)0, tile_rows * row_bytes, 0x00020000);
-  };
-  const __amdgpu_buffer_rsrc_t wr = rsrc(a.qw, a.K / 2), sr = rsrc(a.scales, groups * 2), zr = rsrc(a.zeros, groups);
-  struct Block {
-    uint32_t w[4], s[PER > 1 ? PER / 2 : 1], z;
-  };
-  auto load = [&](Block& x, int b) {
+// Loads the weights of the 16 outputs from n0 on, U blocks at a time: those of outputs >= N and inputs >= K
+// return 0 without an access.
+template <int G, int U> struct W4Weights {
+  static constexpr int NS = U * 128 / G;
+  __amdgpu_buffer_rsrc_t wr, sr, zr;
+  int K, groups, col, j;
+  bool wide, zeros;
+  MQ_DEV W4Weights(const MqW4Args& a, int n0, bool wide_scales, int lane) {
+    K = a.K;
+    groups = K / G;
+    col = lane & 15;
+    j = lane >> 4;
+    wide = wide_scales;
+    zeros = a.zeros != nullptr;
+    const int rows = max(0, min(16, a.N - n0));
+    wr = rsrc(a.qw, K / 2, n0, rows);
+    sr = rsrc(a.scales, groups * 2, n0, rows);
+    zr = rsrc(a.zeros, groups, n0, rows);
+  }
+  static MQ_DEV __amdgpu_buffer_rsrc_t rsrc(const void* p, int row_bytes, int n0, int rows) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)p + (size_t)n0 * row_bytes), (short)0, rows * row_bytes, 0x00020000);
+  }
+  // words of block b
+  MQ_DEV void codes(uint32_t (&w)[4], int b) const {
     const int k = 128 * b + 32 * j;
-    const auto w = __builtin_amdgcn_raw_buffer_load_b128(wr, k < a.K ? col * (a.K / 2) + k / 2 : W4_FAR, 0, 0);
-    for (int i = 0; i < 4; ++i) x.w[i] = w[i];
-    const int g = col * groups + PER * b;
-    x.z = 0x08080808u;
-    if (PER == 1 || pl.wide_scales) {
-      const int so = b < pl.blocks ? 2 * g : W4_FAR;
-      if constexpr (PER == 4) {
-        const auto s = __builtin_amdgcn_raw_buffer_load_b64(sr, so, 0, 0);
-        x.s[0] = s[0];
-        x.s[1] = s[1];
-      } else if constexpr (PER == 2) x.s[0] = __builtin_amdgcn_raw_buffer_load_b32(sr, so, 0, 0);
-      else x.s[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, so, 0, 0);
-      if (a.zeros != nullptr) {
-        const int zo = b < pl.blocks ? g : W4_FAR;
-        if constexpr (PER == 4) x.z = __builtin_amdgcn_raw_buffer_load_b32(zr, zo, 0, 0);
-        else if constexpr (PER == 2) x.z = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(zr, zo, 0, 0);
-        else x.z = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zr, zo, 0, 0);
-      }
-    } else if constexpr (PER > 1) {
-      uint32_t z = 0;
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(wr, k < K ? col * (K / 2) + k / 2 : W4_FAR, 0, 0);
+    for (int i = 0; i < 4; ++i) w[i] = v[i];
+  }
+  // groups of blocks U unit .. U unit + U
+  MQ_DEV void scales(W4Scales<NS>& x, int unit) const {
+    int g = col * groups + NS * unit;
+    asm volatile("" : "+v"(g));          // (opaque: or every group's offset below has a register of its own)
+    for (int i = 0; i < (NS + 3) / 4; ++i) x.z[i] = 0x08080808u;
+    if (wide) {                          // NS groups are there, and aligned
+      if constexpr (NS == 1) x.s[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, 2 * g, 0, 0);
+      else if constexpr (NS == 2) x.s[0] = __builtin_amdgcn_raw_buffer_load_b32(sr, 2 * g, 0, 0);
+      else if constexpr (NS == 4) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(sr, 2 * g, 0, 0);
+        x.s[0] = v[0];
+        x.s[1] = v[1];
+      } else {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const bool in = PER * b + i < groups;
+        for (int q = 0; q < NS / 8; ++q) {
+          const auto v = __builtin_amdgcn_raw_buffer_load_b128(sr, 2 * g + 16 * q, 0, 0);
+          for (int i = 0; i < 4; ++i) x.s[4 * q + i] = v[i];
+        }
+      }
+      if (zeros) {
+        if constexpr (NS == 1) x.z[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zr, g, 0, 0);
+        else if constexpr (NS == 2) x.z[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(zr, g, 0, 0);
+        else {
+#pragma unroll
+          for (int q = 0; q < NS / 4; ++q) x.z[q] = __builtin_amdgcn_raw_buffer_load_b32(zr, g + 4 * q, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const bool in = NS * unit + i < groups;
         const uint32_t s = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, in ? 2 * (g + i) : W4_FAR, 0, 0);
         x.s[i / 2] = i & 1 ? x.s[i / 2] | (s << 16) : s;
-        if (a.zeros != nullptr) z |= (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zr, in ? g + i : W4_FAR, 0, 0) << (8 * i);
-      }
-      if (a.zeros != nullptr) x.z = z;
-    }
-  };
-  auto load_step = [&](Block (&x)[U], int step) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) load(x[u], (step * U + u) * pl.kw + kw);
-  };
-
-  // Rows m0 .. m0 + rows of inputs from 128 c0 on, in operand order, and the sums of their groups.
-  auto stage = [&](int c0) {
-    const int blocks = min(cblocks, pl.blocks - c0), pieces = blocks * 16;
-    for (int id = tid; id < rows * pieces; id += W4_THREADS) {
-      const int m = id / pieces, q = id - m * pieces, b = q >> 4, k = (c0 + b) * 128 + 8 * (q & 15);
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (k < a.K) v = ld16(a.x + (size_t)(m0 + m) * a.K + k);
-      *(uint4*)(xs + (size_t)m * xstride + b * 128 + 8 * w4_slot<G>(q & 15)) = nb_order8(v);
-      float s = nb_sum8<F16>(v);
-      s += dpp_f<MQ_DPP_QUAD_XOR1>(s);
-      s += dpp_f<MQ_DPP_QUAD_XOR2>(s);
-      if constexpr (G >= 64) s += dpp_f<MQ_DPP_ROW_HALF_MIRROR>(s);
-      if constexpr (G >= 128) s += dpp_f<MQ_DPP_ROW_MIRROR>(s);
-      if ((q & (G / 8 - 1)) == 0) xsum[(size_t)(q / (G / 8)) * (16 * MT) + m] = s;
-    }
-  };
-
-  nb_f32x4 acc[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
-  int xrow[MT];                          // (rows past the last read it again; their results are not stored)
-#pragma unroll
-  for (int t = 0; t < MT; ++t) xrow[t] = (ONE ? 0 : min(16 * t + col, rows - 1)) * xstride + 8 * j;
-  const bool s16 = a.s_type == MQ_T_F16;
-
-  auto compute = [&](const Block& x, int b) {        // b: block of the staged ones
-    uint32_t d[4] = {x.w[0], x.w[1], x.w[2], x.w[3]};
-    w4_exchange<G>(d);
-#pragma unroll
-    for (int g = 0; g < PER; ++g) {
-      const float z = -NB_OFFSET - (float)((x.z >> (8 * g)) & 255u);
-      const float* sums = xsum + (size_t)(b * PER + g) * (16 * MT) + (ONE ? 0 : 4 * j);
-      nb_f32x4 c[MT];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if constexpr (ONE) c[t] = nb_f32x4{z * sums[0], 0.f, 0.f, 0.f};
-        else c[t] = *(const nb_f32x4*)(sums + 16 * t) * z;
-      }
-#pragma unroll
-      for (int s = 4 / PER * g; s < 4 / PER * (g + 1); ++s) {
-        const uint4 w = nb_expand8<F16>(d[s]);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) c[t] = nb_mfma<F16>(*(const uint4*)(xs + xrow[t] + b * 128 + 32 * s), w, c[t]);
-      }
-      const float sc = w4_from16((x.s[g / 2] >> (16 * (g & 1))) & 0xffffu, s16);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if constexpr (ONE) acc[t][0] = fmaf(sc, c[t][0], acc[t][0]);
-        else
-          for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(sc, c[t][i], acc[t][i]);
+        if (zeros) {
+          const uint32_t z = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zr, in ? g + i : W4_FAR, 0, 0);
+          x.z[i / 4] = i & 3 ? x.z[i / 4] | (z << (8 * (i & 3))) : z;
+        }
       }
     }
-  };
-
-  Block cur[U];
-  load_step(cur, 0);
-  for (int step = 0; step < pl.steps; ++step) {
-    Block nxt[U];
-    const int c0 = step / pl.chunk * pl.chunk * U * pl.kw;
-    if (step % pl.chunk == 0) {
-      if (step > 0) __syncthreads();
-      stage(c0);
-      __syncthreads();
-    }
-    if (step + 1 < pl.steps) load_step(nxt, step + 1);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int b = (step * U + u) * pl.kw + kw;
-      if (b < pl.blocks) compute(cur[u], b - c0);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) cur[u] = nxt[u];
   }
+};
 
-  // Results: column col is output n0 + col, register i of tile t row 16 t + 4 j + i
-  auto write = [&](int m, int n, float v) {
-    if (m >= rows || n >= a.N) return;
-    const size_t at = (size_t)(m0 + m) * a.N + n;
-    if (a.residual != nullptr) v += w4_residual(a.residual, at, a.o_type);
-    w4_store(a.out, at, v, a.o_type);
-  };
-  if (pl.kw == 1) {
+// acc[t] += the products of a block whose first group is the first-th of sc; x_of(t, step) is the operand of
+// row tile t.  A step's operands are read one step ahead, and no further: steps mixed by the scheduler
+// take more registers than there are.
+template <bool F16, int G, int MT, bool ONE, int NS, class X>
+MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& sc, int first, bool s16, X x_of) {
+  constexpr int SPG = G / 32;            // steps of a group
+  w4_exchange<G>(d);
+  uint4 x[MT], zero;
+  nb_f32x4 c[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) x[t] = x_of(t, 0);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    uint4 xn[MT];
+    if (s < 3) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xn[t] = x_of(t, s + 1);
+    }
+    const int g = first + s / SPG;
+    if (s % SPG == 0) {
+      uint32_t zw = sc.z[g / 4];
+      asm volatile("" : "+v"(zw));
+      const uint32_t z = (zw >> (8 * (g & 3))) & 255u, zc = F16 ? 0xcc00u + (z << 6) : 0xc180u + (z << 3);
+      const uint32_t zz = zc | (zc << 16);                    // -(16 + z), twice
+      zero = make_uint4(zz, zz, zz, zz);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) c[t] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const uint4 w = nb_expand8<F16>(d[s]);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      c[t] = nb_mfma<F16>(x[t], zero, c[t]);
+      c[t] = nb_mfma<F16>(x[t], w, c[t]);
+    }
+    if (s % SPG == SPG - 1) {
+      uint32_t sw = sc.s[g / 2];
+      asm volatile("" : "+v"(sw));       // (opaque: or all groups' scales are converted at the start)
+      const float f = w4_from16((sw >> (16 * (g & 1))) & 0xffffu, s16);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < (ONE ? 1 : 4); ++i) acc[t][i] = fmaf(f, c[t][i], acc[t][i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) x[t] = xn[t];
+  }
+}
+
+// Joins the kw waves of every tile of outputs and writes: column col is output n0 + col, register i of
+// row tile t row 16 t + 4 j + i.
+template <int MT, bool ONE>
+MQ_DEV void w4_finish(const MqW4Args& a, const nb_f32x4 (&acc)[MT], int m0, int rows, int wave, int kw, float* red) {
+  constexpr int R = ONE ? 1 : 4;
+  const int tid = threadIdx.x, lane = tid & 63, tiles = (blockDim.x >> 6) / kw, first = blockIdx.x * tiles * 16;
+  if (kw == 1) {
+    const int n = first + 16 * wave + (lane & 15);
+    if (n >= a.N) return;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int i = 0; i < (ONE ? 1 : 4); ++i) write(16 * t + 4 * j + i, n0 + col, acc[t][i]);
+      for (int i = 0; i < R; ++i) {
+        const int m = 16 * t + 4 * (lane >> 4) + i;
+        if (m < rows) w4_write(a, m0 + m, n, acc[t][i]);
+      }
     return;
   }
-  __syncthreads();
-  constexpr int R = ONE ? 1 : 4;
-  float* red = (float*)lds;              // [wave][MT][R][64]
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int i = 0; i < R; ++i) red[((wave * MT + t) * R + i) * 64 + lane] = acc[t][i];
   __syncthreads();
-  for (int id = tid; id < W4_WAVES / pl.kw * MT * R * 64; id += W4_THREADS) {
-    const int ln = id & 63, v = id >> 6, t = v / R % MT, i = v % R, w = v / (R * MT);
+  for (int id = tid; id < tiles * MT * R * 64; id += blockDim.x) {
+    const int ln = id & 63, v = id >> 6, i = v % R, t = v / R % MT, w = v / (R * MT);
+    const int m = 16 * t + 4 * (ln >> 4) + i, n = first + 16 * w + (ln & 15);
+    if (m >= rows || n >= a.N) continue;
     float sum = 0.f;
-    for (int q = 0; q < pl.kw; ++q) sum += red[(((w * pl.kw + q) * MT + t) * R + i) * 64 + ln];
-    write(16 * t + 4 * (ln >> 4) + i, (blockIdx.x * (W4_WAVES / pl.kw) + w) * 16 + (ln & 15), sum);
+    for (int q = 0; q < kw; ++q) sum += red[(((w * kw + q) * MT + t) * R + i) * 64 + ln];
+    w4_write(a, m0 + m, n, sum);
   }
+}
+
+// Up to 16 rows; wave w takes blocks w, w + 8, .. of the workgroup's 16 outputs.
+template <bool F16, int G, bool ONE>
+__global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bool wide_scales) {
+  constexpr int U = 3;                  // blocks in flight, with their pieces of x
+  typedef W4Weights<G, 1> Weights;
+  __shared__ float red[W4_WAVES * (ONE ? 1 : 4) * 64];
+  const int lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4, blocks = (a.K + 127) / 128;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Weights wt(a, blockIdx.x * 16, wide_scales, lane);
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, (short)0, a.M * a.K * 2, 0x00020000);
+  const int xrow = (ONE ? 0 : min(col, a.M - 1)) * a.K;      // (rows past the last read it again)
+  struct Stretch {
+    uint32_t w[4];
+    W4Scales<Weights::NS> sc;
+    uint4 x[4];
+  };
+  auto load = [&](Stretch& y, int b) {
+    wt.codes(y.w, b);
+    wt.scales(y.sc, b);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = 128 * b + 8 * w4_piece<G>(s, j);
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, k < a.K ? 2 * (xrow + k) : W4_FAR, 0, 0);
+      y.x[s] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+  };
+  nb_f32x4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
+  Stretch y[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (wave + W4_WAVES * u < blocks) load(y[u], wave + W4_WAVES * u);
+  for (int b = wave; b < blocks; b += W4_WAVES * U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (b + W4_WAVES * u < blocks)
+        w4_block<F16, G, 1, ONE>(acc, y[u].w, y[u].sc, 0, a.s_type == MQ_T_F16, [&](int, int s) { return nb_order8(y[u].x[s]); });
+      if (b + W4_WAVES * (u + U) < blocks) load(y[u], b + W4_WAVES * (u + U));
+    }
+  }
+  w4_finish<1, ONE>(a, acc, 0, a.M, wave, W4_WAVES, red);
+}
+
+struct W4Plan {
+  enum { DIRECT, WHOLE, STRETCH } kind;
+  int mt;             // tiles of 16 rows
+  int kw, waves;      // waves that split the inputs, waves of a workgroup
+  int units;          // per wave: w4_unit() blocks each
+  int lds;            // bytes
+  bool wide_scales;   // the scales (and zeros) of a unit (or block, DIRECT) are whole, aligned loads
+};
+
+// Rows of x in LDS, in operand order: [rows][block][step][j][8], rows 16 bytes further apart than their
+// length, so that they start in different banks.
+template <int G> struct W4Rows {
+  const uint16_t* x;
+  int K, rows, per_row, stride;          // 16-byte pieces of a row; elements
+  MQ_DEV W4Rows(const MqW4Args& a, int m0, int rows_, int blocks) {
+    x = a.x + (size_t)m0 * a.K;
+    K = a.K;
+    rows = rows_;
+    per_row = 16 * blocks;
+    stride = 128 * blocks + 8;
+  }
+  // piece `id` of the stretch of inputs that starts at block c0, zeros from K on
+  MQ_DEV uint4 fetch(int id, int c0) const {
+    const int m = id / per_row, k = c0 * 128 + 8 * (id - m * per_row);
+    return k < K ? ld16(x + (size_t)m * K + k) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  MQ_DEV void put(uint16_t* dst, int id, uint4 v) const {
+    const int m = id / per_row, q = id - m * per_row;
+    *(uint4*)(dst + (size_t)m * stride + (q >> 4) * 128 + 8 * w4_slot<G>(q & 15)) = nb_order8(v);
+  }
+  MQ_DEV void all(uint16_t* dst, int c0) const {
+    const int total = rows * per_row, threads = blockDim.x;
+    for (int id = threadIdx.x; id < total; id += 4 * threads) {
+      uint4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (id + i * threads < total) v[i] = fetch(id + i * threads, c0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (id + i * threads < total) put(dst, id + i * threads, v[i]);
+    }
+  }
+};
+
+#define W4_WHOLE_UNIT 4      // blocks of 128 inputs that a wave has in flight
+#define W4_STRETCH_UNIT 2    // blocks per wave and stretch; twice as many in flight
+#define W4_PIECES 8          // 16-byte pieces of x that a thread carries from one stretch to the next
+
+template <bool F16, int G, int MT, bool ONE>
+__global__ void __launch_bounds__(W4_THREADS, MT == 2 ? 2 : G == 32 && !ONE ? 3 : 4) w4_whole_kernel(MqW4Args a, W4Plan pl) {
+  constexpr int U = W4_WHOLE_UNIT;
+  typedef W4Weights<G, U> Weights;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = wave / pl.kw, kw = wave - nw * pl.kw;
+  const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
+  uint16_t* xs = (uint16_t*)lds;
+  const Weights wt(a, (blockIdx.x * (pl.waves / pl.kw) + nw) * 16, pl.wide_scales, lane);
+  const bool s16 = a.s_type == MQ_T_F16;
+  uint32_t w[U][4];
+  W4Scales<Weights::NS> sc;
+#pragma unroll
+  for (int u = 0; u < U; ++u) wt.codes(w[u], kw * U + u);
+  wt.scales(sc, kw);
+  const W4Rows<G> rx(a, m0, rows, pl.units * U * pl.kw);
+  rx.all(xs, 0);
+  nb_f32x4 acc[MT];
+  int xrow[MT];                          // (rows past the last read it again; their results are not stored)
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    acc[t] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
+    xrow[t] = (ONE ? 0 : min(16 * t + col, rows - 1)) * rx.stride + 8 * j;
+  }
+  __syncthreads();
+  for (int i = 0; i < pl.units; ++i) {
+    const bool more = i + 1 < pl.units;
+    const int unit = i * pl.kw + kw, next = unit + pl.kw;
+    W4Scales<Weights::NS> nsc;
+    if (more) wt.scales(nsc, next);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t d[4] = {w[u][0], w[u][1], w[u][2], w[u][3]};
+      if (more) wt.codes(w[u], next * U + u);
+      const uint16_t* at = xs + (unit * U + u) * 128;
+      w4_block<F16, G, MT, ONE>(acc, d, sc, u * (128 / G), s16, [&](int t, int s) { return *(const uint4*)(at + xrow[t] + 32 * s); });
+    }
+    sc = nsc;
+  }
+  if (pl.kw > 1) __syncthreads();
+  w4_finish<MT, ONE>(a, acc, m0, rows, wave, pl.kw, (float*)lds);
+}
+
+template <bool F16, int G, int MT>
+__global__ void __launch_bounds__(W4_THREADS, MT == 1 ? 3 : 2) w4_stretch_kernel(MqW4Args a, W4Plan pl) {
+  constexpr int U = W4_STRETCH_UNIT;
+  typedef W4Weights<G, U> Weights;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = wave / pl.kw, kw = wave - nw * pl.kw;
+  const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
+  const Weights wt(a, (blockIdx.x * (W4_WAVES / pl.kw) + nw) * 16, pl.wide_scales, lane);
+  const bool s16 = a.s_type == MQ_T_F16;
+  const int sblocks = U * pl.kw;                       // blocks of a stretch
+  const W4Rows<G> rx(a, m0, rows, sblocks);
+  uint16_t* xs = (uint16_t*)lds;                       // [2] stretches
+  const int half = rows * rx.stride, total = rows * rx.per_row;
+  // weights of this stretch and the next
+  uint32_t w[2][U][4];
+  W4Scales<Weights::NS> sc[2];
+  auto load = [&](int p, int step) {
+    const int unit = step * pl.kw + kw;
+#pragma unroll
+    for (int u = 0; u < U; ++u) wt.codes(w[p][u], unit * U + u);
+    wt.scales(sc[p], unit);
+  };
+  load(0, 0);
+  if (pl.units > 1) load(1, 1);
+  rx.all(xs, 0);
+  nb_f32x4 acc[MT];
+  int xrow[MT];                          // (rows past the last read it again; their results are not stored)
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    acc[t] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
+    xrow[t] = min(16 * t + col, rows - 1) * rx.stride + 8 * j;
+  }
+  auto stretch = [&](auto p_tag, int step) {
+    constexpr int P = decltype(p_tag)::value;
+    const bool more = step + 1 < pl.units;
+    __syncthreads();
+    // (opaque ids: the compiler would keep every piece's address in a register across the loop)
+    uint4 v[W4_PIECES];
+    if (more) {
+#pragma unroll
+      for (int i = 0; i < W4_PIECES; ++i) {
+        int id = tid + i * W4_THREADS;
+        asm volatile("" : "+v"(id));
+        if (id < total) v[i] = rx.fetch(id, (step + 1) * sblocks);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t d[4] = {w[P][u][0], w[P][u][1], w[P][u][2], w[P][u][3]};
+      const uint16_t* at = xs + P * half + (kw * U + u) * 128;
+      w4_block<F16, G, MT, false>(acc, d, sc[P], u * (128 / G), s16, [&](int t, int s) { return *(const uint4*)(at + xrow[t] + 32 * s); });
+    }
+    if (step + 2 < pl.units) load(P, step + 2);
+    if (more) {                          // (the readers of that half passed the barrier above)
+#pragma unroll
+      for (int i = 0; i < W4_PIECES; ++i) {
+        int id = tid + i * W4_THREADS;
+        asm volatile("" : "+v"(id));
+        if (id < total) rx.put(xs + (1 - P) * half, id, v[i]);
+      }
+    }
+  };
+  for (int step = 0; step < pl.units; step += 2) {
+    stretch(std::integral_constant<int, 0>(), step);
+    if (step + 1 < pl.units) stretch(std::integral_constant<int, 1>(), step + 1);
+  }
+  if (pl.kw > 1) __syncthreads();
+  w4_finish<MT, false>(a, acc, m0, rows, wave, pl.kw, (float*)lds);
+}
+
+W4Plan w4_plan(const MqW4Args& a) {
+  W4Plan p;
+  const int tiles = (a.N + 15) / 16, blocks = (a.K + 127) / 128, rows = a.M < 64 ? a.M : 64;
+  p.mt = (rows + 15) / 16;
+  p.waves = a.M == 1 ? 4 : W4_WAVES;
+  // All of K in LDS if two workgroups of it fit a compute unit
+  p.kind = a.M <= 16 && tiles <= 512 ? W4Plan::DIRECT
+           : p.mt <= 2 && (long long)rows * a.K * 2 <= 65536 ? W4Plan::WHOLE : W4Plan::STRETCH;
+  if (p.kind == W4Plan::STRETCH) p.waves = W4_WAVES;
+  const int unit = p.kind == W4Plan::DIRECT ? 1 : p.kind == W4Plan::WHOLE ? W4_WHOLE_UNIT : W4_STRETCH_UNIT;
+  const int ns = unit * 128 / a.G;       // groups loaded at a time
+  p.wide_scales = a.K % (ns * a.G) == 0 && ((uintptr_t)a.scales & 15) == 0 && ((uintptr_t)a.zeros & 15) == 0;
+  // Waves that split the inputs leave fewer outputs to share x: as many as fill the chip (16 waves per
+  // compute unit, 8 of the kernels with more registers)
+  const long long most = p.mt <= 2 ? 4096 : 2048;
+  p.kw = p.waves;
+  while (p.kw > 1 && (tiles * p.kw > most || unit * (p.kw / 2) >= blocks ||
+                      (p.kind == W4Plan::STRETCH && rows * 16 * unit * p.kw > W4_PIECES * W4_THREADS)))
+    p.kw /= 2;
+  p.units = (blocks + unit * p.kw - 1) / (unit * p.kw);
+  const int held = p.kind == W4Plan::WHOLE ? p.units * unit * p.kw : unit * p.kw, red = p.kw > 1 ? p.waves * p.mt * 1024 : 0;
+  const int x = (p.kind == W4Plan::WHOLE ? 1 : 2) * rows * (held * 256 + 16);
+  p.lds = x > red ? x : red;
+  return p;
 }
 
 }  // namespace
 
 int mq_launch_w4_linear(const MqW4Args& a, hipStream_t stream) {
-  const int mt = a.M > 48 ? 4 : (a.M + 15) / 16, rows = a.M < 16 * mt ? a.M : 16 * mt;
-  const long long tiles = (a.N + 15) / 16;
-  const int unroll = w4_unroll(mt);
-  W4Plan p;
-  p.blocks = (a.K + 127) / 128;
-  p.kw = W4_WAVES;
-  while (p.kw > 1 && (tiles * p.kw > 4096 || p.kw > p.blocks)) p.kw /= 2;
-  p.steps = (p.blocks + unroll * p.kw - 1) / (unroll * p.kw);
-  // x and its sums of some steps: rows * (256 blocks + 16 of padding) + 4 * 16 mt * (128 / G) blocks
-  auto bytes = [&](int chunk) {
-    const size_t blocks = (size_t)chunk * unroll * p.kw;
-    return ((size_t)rows * (blocks * 256 + 16) + 15) / 16 * 16 + blocks * (128 / a.G) * 64 * mt;
-  };
-  while (p.kw > 1 && bytes(1) > W4_LDS) {
-    p.kw /= 2;
-    p.steps = (p.blocks + unroll * p.kw - 1) / (unroll * p.kw);
-  }
-  p.chunk = 1;
-  while (p.chunk < p.steps && bytes(p.chunk + 1) <= W4_LDS) ++p.chunk;
-  const size_t red = p.kw > 1 ? (size_t)W4_WAVES * mt * 1024 : 0;
-  p.lds = (int)(bytes(p.chunk) > red ? bytes(p.chunk) : red);
-  p.wide_scales = a.K % 128 == 0 && ((uintptr_t)a.scales & 7) == 0 && ((uintptr_t)a.zeros & 3) == 0;
-  const int per = W4_WAVES / p.kw;
-  const unsigned gx = (unsigned)((tiles + per - 1) / per);
+  const W4Plan p = w4_plan(a);
+  const int per = 16 * (p.waves / p.kw);                         // outputs of a workgroup
+  const unsigned gx = (unsigned)(((long long)a.N + per - 1) / per);
   auto go = [&](auto f16, auto g) {
     constexpr bool F = decltype(f16)::value;
     constexpr int G = decltype(g)::value;
-    for (int m0 = 0; m0 < a.M; m0 += 65535 * 64) {          // the grid's second dimension
+    if (p.kind == W4Plan::DIRECT) {
+      const dim3 grid((a.N + 15) / 16);
+      if (a.M == 1) hipLaunchKernelGGL((w4_direct_kernel<F, G, true>), grid, dim3(W4_THREADS), 0, stream, a, p.wide_scales);
+      else hipLaunchKernelGGL((w4_direct_kernel<F, G, false>), grid, dim3(W4_THREADS), 0, stream, a, p.wide_scales);
+      return;
+    }
+    for (int m0 = 0; m0 < a.M; m0 += 65535 * 64) {               // the grid's second dimension
       MqW4Args b = a;
       const size_t out = a.o_type == MQ_T_F32 ? 4 : 2;
       b.x = a.x + (size_t)m0 * a.K;
       b.out = (char*)a.out + (size_t)m0 * a.N * out;
       if (a.residual != nullptr) b.residual = (const char*)a.residual + (size_t)m0 * a.N * out;
       b.M = a.M - m0 < 65535 * 64 ? a.M - m0 : 65535 * 64;
-      const dim3 grid(gx, (unsigned)((b.M + 16 * mt - 1) / (16 * mt)));
-      if (b.M == 1 && mt == 1) hipLaunchKernelGGL((w4_kernel<F, G, 1, true>), grid, dim3(W4_THREADS), p.lds, stream, b, p);
-      else if (mt == 1) hipLaunchKernelGGL((w4_kernel<F, G, 1, false>), grid, dim3(W4_THREADS), p.lds, stream, b, p);
-      else if (mt == 2) hipLaunchKernelGGL((w4_kernel<F, G, 2, false>), grid, dim3(W4_THREADS), p.lds, stream, b, p);
-      else if (mt == 3) hipLaunchKernelGGL((w4_kernel<F, G, 3, false>), grid, dim3(W4_THREADS), p.lds, stream, b, p);
-      else hipLaunchKernelGGL((w4_kernel<F, G, 4, false>), grid, dim3(W4_THREADS), p.lds, stream, b, p);
+      const dim3 grid(gx, (unsigned)((b.M + 16 * p.mt - 1) / (16 * p.mt)));
+      auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * p.waves), p.lds, stream, b, p); };
+      if (p.kind == W4Plan::WHOLE) launch(a.M == 1 ? w4_whole_kernel<F, G, 1, true> : p.mt == 1 ? w4_whole_kernel<F, G, 1, false> : w4_whole_kernel<F, G, 2, false>);
+      else launch(p.mt == 1 ? w4_stretch_kernel<F, G, 1> : p.mt == 2 ? w4_stretch_kernel<F, G, 2> : p.mt == 3 ? w4_stretch_kernel<F, G, 3> : w4_stretch_kernel<F, G, 4>);
     }
   };
   auto pick = [&](auto f16) {
