@@ -121,12 +121,46 @@ struct AtArgs {
   float scale_log2;
 };
 
+// 16 bits of a word as the upper half of an fp32 (a bf16 scale), chosen by a byte selector
+MQ_DEV float at_pick(uint32_t hi, uint32_t lo, uint32_t sel) { return __uint_as_float(__builtin_amdgcn_perm(hi, lo, sel)); }
+MQ_DEV float at_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }    // (fmaxf canonicalises its operands first)
+// a + a's value in the lane that DPP control CTRL names
+template <int CTRL> MQ_DEV float at_add_dpp(float a) {
+#pragma clang fp contract(off)
+  return a + dpp_f<CTRL>(a);
+}
+// a b, and 0 where a or b is 0 whatever the other: a masked position's weight is 0, its scale may be NaN.
+// (The instruction by its intrinsic: between transcendentals and matrix products the compiler has to place
+// wait states, which it does not for instructions written as inline assembly.)
+extern "C" __device__ float at_mul0(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+// Two weights as the truncated bf16 and the bf16 of the remainder
+MQ_DEV void at_split2(float w0, float w1, uint32_t& hi, uint32_t& lo) {
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  hi = __builtin_amdgcn_perm(__float_as_uint(w1), __float_as_uint(w0), 0x07060302u);
+  // w - hi as a two-element product with (-1, 0) and (0, -1), in registers that the compiler cannot see
+  // through: as a constant it would encode (-1, 0) as -1.0, which the hardware reads as (0, -1)
+  uint32_t c0 = 0x0000bf80u, c1 = 0xbf800000u;
+  asm("" : "+s"(c0), "+s"(c1));
+  const v2 h = __builtin_bit_cast(v2, hi);
+  const f2 r = {__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(v2, c0), w0, false),
+                __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(v2, c1), w1, false)};
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2));
+}
+
+// 32 positions as a lane holds them: K words of position 16 t + col, dims (D / 4) j + ..; value dims
+// DPL col + .. and scales of positions 16 t + 4 j + i.
+template <int D, int NG> struct AtTile {
+  uint32_t k[2][D / 32], v[8], s[NG == 4 ? 16 : NG == 2 ? 16 : 8];
+};
+
 template <bool F16, int D, int NG, int CT>
-__global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) {
-  constexpr int KW = D / 32;       // words of a key row per lane: dims (D / 4) j + 8 s + ..
+__global__ void __launch_bounds__(64 * AT_WAVES, CT == 1 ? 3 : 2) kv4_attend_kernel(AtArgs a) {
+  constexpr int KW = D / 32;       // words of a key row per lane
   constexpr int DPL = D / 16;      // dims of a value row per lane
   constexpr int RQ = 16 / NG;      // query rows per column tile
   constexpr int G = D / NG;
+  typedef AtTile<D, NG> Tile;
   __shared__ float red[AT_WAVES][4 * DPL][64];
   __shared__ float2 red_ml[AT_WAVES][CT][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -144,11 +178,16 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
   const int end = limit(min(r0 + CT * RQ, rows) - 1), sure = limit(r0);
   const int chunk = ((end + a.nsplit - 1) / a.nsplit + AT_TILE - 1) / AT_TILE * AT_TILE;
   const int p0 = split * chunk, p1 = min(end, p0 + chunk);
+  // scores are taken with the scale's sign in the queries, so that the largest stays the largest; a scale
+  // of 0 is one next to it, so that a masked score, -inf, stays -inf
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
 
   uint4 qf[CT][KW];
-  float cinit[CT], m[CT], l[CT], sv[CT];
+  // m: a column's reference point (lowest: none yet), l: its sum of weights in this lane's positions
+  float cinit[CT], m[CT], l[CT];
   int lim[CT];
-  nb_f32x4 acc[CT][DPL];
+  nb_f32x4 acc[CT][DPL], sv[CT];   // sv: the sums of the weights times the value scales, in every row
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int r = r0 + ct * RQ + col / NG;
@@ -160,14 +199,18 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
     for (int s = 0; s < KW; ++s) {
       const int d = (D / 4) * j + 8 * s;
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (there && d / G == g) x = nb_order8(nb_load16(qr + d));
+      if (there && d / G == g) {
+        x = nb_order8(nb_load16(qr + d));
+        x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+      }
       qf[ct][s] = x;
       sum += nb_sum8<F16>(x);
     }
     cinit[ct] = -AT_BIAS * sum_xor32(sum_xor16(sum));
     lim[ct] = there ? limit(r) : 0;
-    m[ct] = -INFINITY;
-    l[ct] = sv[ct] = 0.f;
+    m[ct] = -3.402823466e38f;
+    l[ct] = 0.f;
+    sv[ct] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < DPL; ++i) acc[ct][i] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -178,9 +221,6 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
     return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + row * row_bytes), (short)0, end * row_bytes, 0x00020000);
   };
   const __amdgpu_buffer_rsrc_t kr = rsrc(a.c.kq, D / 2), vr = rsrc(a.c.vq, D / 2), sr = rsrc(a.c.scales, 4 * NG);
-  struct Tile {
-    uint32_t k[2][KW], v[8], ks[8], vs[8];
-  };
   auto load = [&](Tile& x, int p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -192,25 +232,43 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
         const auto w = __builtin_amdgcn_raw_buffer_load_b64(kr, ko, 0, 0);
         for (int s = 0; s < 2; ++s) x.k[t][s] = w[s];
       }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if constexpr (NG == 1) {           // (key, value) scale pairs of 4 positions
+        const auto w = __builtin_amdgcn_raw_buffer_load_b128(sr, (p + 16 * t + 4 * j) * 4, 0, 0);
+        for (int i = 0; i < 4; ++i) x.s[4 * t + i] = w[i];
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int pos = p + 16 * t + 4 * j + i, e = 4 * t + i;
+        if constexpr (NG == 2) {         // both groups of key and value
+          const auto w = __builtin_amdgcn_raw_buffer_load_b64(sr, pos * 8, 0, 0);
+          x.s[2 * e] = w[0];
+          x.s[2 * e + 1] = w[1];
+        } else if constexpr (NG == 4) {
+          x.s[2 * e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * 16 + 2 * g, 0, 0);
+          x.s[2 * e + 1] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * 16 + 8 + 2 * g, 0, 0);
+        }
         if constexpr (DPL == 8) x.v[e] = __builtin_amdgcn_raw_buffer_load_b32(vr, pos * (D / 2) + 4 * col, 0, 0);
         else x.v[e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vr, pos * (D / 2) + 2 * col, 0, 0);
-        if constexpr (NG == 1) {
-          const uint32_t w = __builtin_amdgcn_raw_buffer_load_b32(sr, pos * 4, 0, 0);
-          x.ks[e] = w << 16;
-          x.vs[e] = w & 0xffff0000u;
-        } else {
-          x.ks[e] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * (4 * NG) + 2 * g, 0, 0) << 16;
-          x.vs[e] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * (4 * NG) + 2 * NG + 2 * g, 0, 0) << 16;
-        }
       }
     }
   };
+  const uint32_t half = NG == 2 && g == 1 ? 0x03020c0cu : 0x01000c0cu;      // (0x0c: a zero byte)
+  auto key_scale = [&](const Tile& x, int e) {
+    if constexpr (NG == 1) return __uint_as_float(x.s[e] << 16);
+    else if constexpr (NG == 2) return at_pick(x.s[2 * e], x.s[2 * e], half);
+    else return __uint_as_float(x.s[2 * e] << 16);
+  };
+  auto value_scale = [&](const Tile& x, int e) {
+    if constexpr (NG == 1) return __uint_as_float(x.s[e] & 0xffff0000u);
+    else if constexpr (NG == 2) return at_pick(x.s[2 * e + 1], x.s[2 * e + 1], half);
+    else return __uint_as_float(x.s[2 * e + 1] << 16);
+  };
 
   auto step = [&](const Tile& x, int p) {
-    // scores z[ct][e] (log2 units) of positions p + 16 (e / 4) + 4 j + e % 4
+    // scores z[ct][e], not yet scaled, of positions p + 16 (e / 4) + 4 j + e % 4
     float z[CT][8];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -224,28 +282,34 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
         for (int ct = 0; ct < CT; ++ct) s[ct] = nb_mfma<F16>(kx, qf[ct][w], s[ct]);
       }
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+      for (int i = 0; i < 4; ++i) {
+        const float ks = key_scale(x, 4 * t + i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = s[ct][i] * __uint_as_float(x.ks[4 * t + i]);
-          if constexpr (NG >= 2) v += dpp_f<MQ_DPP_QUAD_XOR1>(v);
-          if constexpr (NG >= 4) v += dpp_f<MQ_DPP_QUAD_XOR2>(v);
-          z[ct][4 * t + i] = v * a.scale_log2;
+        for (int ct = 0; ct < CT; ++ct) {
+          float v = s[ct][i] * ks;
+          if constexpr (NG >= 2) v = at_add_dpp<MQ_DPP_QUAD_XOR1>(v);
+          if constexpr (NG >= 4) v = at_add_dpp<MQ_DPP_QUAD_XOR2>(v);
+          z[ct][4 * t + i] = v;
         }
+      }
     }
     if (p + AT_TILE > sure) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 8; ++e) {
           if (p + 16 * (e >> 2) + 4 * j + (e & 3) >= lim[ct]) z[ct][e] = -INFINITY;
+          asm volatile("" : "+v"(z[ct][e]));     // (keeps this a branch: few tiles need it)
+        }
     }
     uint4 ph[CT], pl[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      float mt = fmaxf(fmaxf(fmaxf(z[ct][0], z[ct][1]), fmaxf(z[ct][2], z[ct][3])),
-                       fmaxf(fmaxf(z[ct][4], z[ct][5]), fmaxf(z[ct][6], z[ct][7])));
-      mt = max_xor32(max_xor16(mt));
+      float mt = at_max(at_max(at_max(z[ct][0], z[ct][1]), z[ct][2]), at_max(at_max(z[ct][3], z[ct][4]), at_max(z[ct][5], at_max(z[ct][6], z[ct][7]))));
+      float2 pr = swap16(mt);
+      mt = at_max(pr.x, pr.y);
+      pr = swap32(mt);
+      mt = at_max(pr.x, pr.y) * scale;
       if (__builtin_amdgcn_ballot_w64(mt > m[ct] + AT_RAISE) != 0) {
         const bool up = mt > m[ct] + AT_RAISE;
         const float alpha = up ? __builtin_amdgcn_exp2f(m[ct] - mt) : 1.0f;
@@ -255,27 +319,24 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
 #pragma unroll
         for (int i = 0; i < DPL; ++i) acc[ct][i] *= alpha;
       }
-      // (nothing seen yet: every weight of the column is 2^-inf)
-      const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         float w[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float p_ = __builtin_amdgcn_exp2f(z[ct][e + i] - ref);
+          const float p_ = __builtin_amdgcn_exp2f(fmaf(z[ct][e + i], scale, -m[ct]));
           l[ct] += p_;
-          // a masked position's scale may be anything
-          w[i] = z[ct][e + i] == -INFINITY ? 0.f : p_ * __uint_as_float(x.vs[e + i]);
-          sv[ct] += w[i];
+          w[i] = at_mul0(p_, value_scale(x, e + i));
         }
-        hi[e / 2] = __builtin_amdgcn_perm(__float_as_uint(w[1]), __float_as_uint(w[0]), 0x07060302u);
-        lo[e / 2] = (uint32_t)f32_to_bf16(w[0] - __uint_as_float(__float_as_uint(w[0]) & 0xffff0000u)) |
-                    ((uint32_t)f32_to_bf16(w[1] - __uint_as_float(__float_as_uint(w[1]) & 0xffff0000u)) << 16);
+        at_split2(w[0], w[1], hi[e / 2], lo[e / 2]);
       }
       ph[ct] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       pl[ct] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
+    const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) sv[ct] = nb_mfma<false>(ones, pl[ct], nb_mfma<false>(ones, ph[ct], sv[ct]));
     // value codes of position pairs in the halves of a word: words f of wl hold dims DPL col + f
     uint32_t wl[4], wh[4];
 #pragma unroll
@@ -303,17 +364,16 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
       values(std::integral_constant<int, 3>(), wh, 7);
     }
   };
-
+  constexpr int STRIDE = AT_TILE * AT_WAVES;
+  Tile x, y;
   int p = p0 + AT_TILE * wave;
-  if (p < p1) {
-    Tile x;
-    load(x, p);
-    for (; p < p1; p += AT_TILE * AT_WAVES) {
-      Tile y;
-      load(y, p + AT_TILE * AT_WAVES);       // (past the end: zeros, not used)
-      step(x, p);
-      x = y;
-    }
+  if (p < p1) load(x, p);
+  for (; p < p1; p += 2 * STRIDE) {          // (loads past the end: zeros, not used)
+    load(y, p + STRIDE);
+    step(x, p);
+    if (p + STRIDE >= p1) break;
+    load(x, p + 2 * STRIDE);
+    step(y, p + STRIDE);
   }
 
   // Join the waves.  A column's O, without the codes' offset, is in value order i' DPL + i, where
@@ -321,7 +381,6 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     l[ct] = sum_xor32(sum_xor16(l[ct]));
-    sv[ct] = sum_xor32(sum_xor16(sv[ct]));
     if (j == 0) red_ml[wave][ct][col] = make_float2(m[ct], l[ct]);
   }
 #pragma unroll
@@ -330,7 +389,7 @@ __global__ void __launch_bounds__(64 * AT_WAVES, 2) kv4_attend_kernel(AtArgs a) 
 #pragma unroll
     for (int i = 0; i < DPL; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[wave][e * DPL + i][lane] = fmaf(-AT_BIAS, sv[ct], acc[ct][i][e]);
+      for (int e = 0; e < 4; ++e) red[wave][e * DPL + i][lane] = fmaf(-AT_BIAS, sv[ct][e], acc[ct][i][e]);
     __syncthreads();
     float mx = -INFINITY, sum = 0.f, f[AT_WAVES];
 #pragma unroll

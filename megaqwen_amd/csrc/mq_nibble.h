@@ -18,10 +18,13 @@ typedef float nb_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 nb_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 nb_f16x8 __attribute__((ext_vector_type(8)));
 
-// Codes F and F + 4 of a word (bits 4F.. and 16 + 4F..) as the elements 16 + u.
+// Codes F and F + 4 of a word (bits 4F.. and 16 + 4F..) as the elements 16 + u.  The constants are in
+// registers that the compiler cannot see through: as literals, the and and the or are an instruction each.
 template <bool F16, int F> MQ_DEV uint32_t nb_pair(uint32_t w) {
   constexpr int at = F16 ? 6 : 3, sh = 4 * F - at;
-  const uint32_t m = F16 ? 0x03c003c0u : 0x00780078u, one = F16 ? 0x4c004c00u : 0x41804180u;
+  uint32_t m = F16 ? 0x03c003c0u : 0x00780078u, one = F16 ? 0x4c004c00u : 0x41804180u;
+  asm("" : "+s"(m));
+  asm("" : "+v"(one));
   return ((sh < 0 ? w << (sh < 0 ? -sh : 0) : w >> (sh > 0 ? sh : 0)) & m) | one;
 }
 // The 8 codes of a word as an operand: elements 2f and 2f + 1 are codes f and f + 4.

@@ -154,11 +154,11 @@ template <int G, int U> struct W4Weights {
   }
 };
 
-// acc[t] += the products of a block whose first group is the first-th of sc; x_of(t, step) is the operand of
-// row tile t.  A step's operands are read one step ahead, and no further: steps mixed by the scheduler
+// acc[t] += the products of a block whose first group is the first-th of sc (s16: all ones if the scales are
+// fp16, 0 for bf16); x_of(t, step) is the operand of row tile t.  A step's operands are read one step ahead, and no further: steps mixed by the scheduler
 // take more registers than there are.
 template <bool F16, int G, int MT, bool ONE, int NS, class X>
-MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& sc, int first, bool s16, X x_of) {
+MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& sc, int first, uint32_t s16, X x_of) {
   constexpr int SPG = G / 32;            // steps of a group
   w4_exchange<G>(d);
   uint4 x[MT], zero;
@@ -174,9 +174,7 @@ MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& 
     }
     const int g = first + s / SPG;
     if (s % SPG == 0) {
-      uint32_t zw = sc.z[g / 4];
-      asm volatile("" : "+v"(zw));
-      const uint32_t z = (zw >> (8 * (g & 3))) & 255u, zc = F16 ? 0xcc00u + (z << 6) : 0xc180u + (z << 3);
+      const uint32_t z = (sc.z[g / 4] >> (8 * (g & 3))) & 255u, zc = F16 ? 0xcc00u + (z << 6) : 0xc180u + (z << 3);
       const uint32_t zz = zc | (zc << 16);                    // -(16 + z), twice
       zero = make_uint4(zz, zz, zz, zz);
 #pragma unroll
@@ -189,13 +187,15 @@ MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& 
       c[t] = nb_mfma<F16>(x[t], w, c[t]);
     }
     if (s % SPG == SPG - 1) {
-      uint32_t sw = sc.s[g / 2];
-      asm volatile("" : "+v"(sw));       // (opaque: or all groups' scales are converted at the start)
-      const float f = w4_from16((sw >> (16 * (g & 1))) & 0xffffu, s16);
+      // (both readings and a select: a branch here moves all groups' sums to the end of the block)
+      const uint32_t sw = g & 1 ? sc.s[g / 2] >> 16 : sc.s[g / 2], half = __float_as_uint(w4_from16(sw & 0xffffu, true));
+      const float f = __uint_as_float((half & s16) | ((sw << 16) & ~s16));
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int i = 0; i < (ONE ? 1 : 4); ++i) acc[t][i] = fmaf(f, c[t][i], acc[t][i]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) asm volatile("" : "+v"(acc[t]));      // (here, and not behind the next loads)
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
       y.x[s] = make_uint4(v[0], v[1], v[2], v[3]);
     }
   };
+  const uint32_t s16 = a.s_type == MQ_T_F16 ? ~0u : 0u;
   nb_f32x4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
   Stretch y[U];
 #pragma unroll
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (b + W4_WAVES * u < blocks)
-        w4_block<F16, G, 1, ONE>(acc, y[u].w, y[u].sc, 0, a.s_type == MQ_T_F16, [&](int, int s) { return nb_order8(y[u].x[s]); });
+        w4_block<F16, G, 1, ONE>(acc, y[u].w, y[u].sc, 0, s16, [&](int, int s) { return nb_order8(y[u].x[s]); });
       if (b + W4_WAVES * (u + U) < blocks) load(y[u], b + W4_WAVES * (u + U));
     }
   }
@@ -289,23 +290,25 @@ struct W4Plan {
 
 // Rows of x in LDS, in operand order: [rows][block][step][j][8], rows 16 bytes further apart than their
 // length, so that they start in different banks.
-template <int G> struct W4Rows {
+template <int G, bool POW2> struct W4Rows {
   const uint16_t* x;
-  int K, rows, per_row, stride;          // 16-byte pieces of a row; elements
+  int K, rows, per_row, stride;          // 16-byte pieces of a row (POW2: a power of two); elements
+  int shift;
   MQ_DEV W4Rows(const MqW4Args& a, int m0, int rows_, int blocks) {
     x = a.x + (size_t)m0 * a.K;
     K = a.K;
     rows = rows_;
     per_row = 16 * blocks;
+    shift = 31 - __builtin_clz(per_row);
     stride = 128 * blocks + 8;
   }
   // piece `id` of the stretch of inputs that starts at block c0, zeros from K on
   MQ_DEV uint4 fetch(int id, int c0) const {
-    const int m = id / per_row, k = c0 * 128 + 8 * (id - m * per_row);
+    const int m = POW2 ? id >> shift : id / per_row, k = c0 * 128 + 8 * (id - m * per_row);
     return k < K ? ld16(x + (size_t)m * K + k) : make_uint4(0u, 0u, 0u, 0u);
   }
   MQ_DEV void put(uint16_t* dst, int id, uint4 v) const {
-    const int m = id / per_row, q = id - m * per_row;
+    const int m = POW2 ? id >> shift : id / per_row, q = id - m * per_row;
     *(uint4*)(dst + (size_t)m * stride + (q >> 4) * 128 + 8 * w4_slot<G>(q & 15)) = nb_order8(v);
   }
   MQ_DEV void all(uint16_t* dst, int c0) const {
@@ -336,13 +339,13 @@ __global__ void __launch_bounds__(W4_THREADS, MT == 2 ? 2 : G == 32 && !ONE ? 3 
   const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
   uint16_t* xs = (uint16_t*)lds;
   const Weights wt(a, (blockIdx.x * (pl.waves / pl.kw) + nw) * 16, pl.wide_scales, lane);
-  const bool s16 = a.s_type == MQ_T_F16;
+  const uint32_t s16 = a.s_type == MQ_T_F16 ? ~0u : 0u;
   uint32_t w[U][4];
   W4Scales<Weights::NS> sc;
 #pragma unroll
   for (int u = 0; u < U; ++u) wt.codes(w[u], kw * U + u);
   wt.scales(sc, kw);
-  const W4Rows<G> rx(a, m0, rows, pl.units * U * pl.kw);
+  const W4Rows<G, false> rx(a, m0, rows, pl.units * U * pl.kw);
   rx.all(xs, 0);
   nb_f32x4 acc[MT];
   int xrow[MT];                          // (rows past the last read it again; their results are not stored)
@@ -379,9 +382,9 @@ __global__ void __launch_bounds__(W4_THREADS, MT == 1 ? 3 : 2) w4_stretch_kernel
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = wave / pl.kw, kw = wave - nw * pl.kw;
   const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
   const Weights wt(a, (blockIdx.x * (W4_WAVES / pl.kw) + nw) * 16, pl.wide_scales, lane);
-  const bool s16 = a.s_type == MQ_T_F16;
+  const uint32_t s16 = a.s_type == MQ_T_F16 ? ~0u : 0u;
   const int sblocks = U * pl.kw;                       // blocks of a stretch
-  const W4Rows<G> rx(a, m0, rows, sblocks);
+  const W4Rows<G, true> rx(a, m0, rows, sblocks);
   uint16_t* xs = (uint16_t*)lds;                       // [2] stretches
   const int half = rows * rx.stride, total = rows * rx.per_row;
   // weights of this stretch and the next
