@@ -85,31 +85,28 @@ class KV4Cache:
         self.head_dim, self.device = 2 * half, k_codes.device
         self.group_size = self.head_dim // scales.shape[-1]
         self._dev = k_codes.get_device()
-        self._lib = _lib.load()
+        lib = _lib.load()
+        self._append, self._read, self._attend = lib.mq_kv4_append, lib.mq_kv4_read, lib.mq_kv4_attend
+        self._workspace = lib.mq_kv4_attend_workspace_bytes
         self._desc = _lib.Kv4Cache(k_codes.data_ptr(), v_codes.data_ptr(), scales.data_ptr(), self.batch,
                                    self.num_kv_heads, self.max_seq_len, self.head_dim, self.group_size)
         self._ref = ctypes.byref(self._desc)
 
     # ------------------------------------------------------------------------------ checks
-    def _rows(self, what: str, name: str, x: torch.Tensor, heads: Optional[int], like=None):
-        """x as [batch, t, heads, head_dim] with a contiguous last dimension, and its strides."""
-        if x.device != self.device:
+    def _rows(self, what: str, name: str, x: torch.Tensor, heads: Optional[int]):
+        """x as [batch, t, heads, head_dim] with a contiguous last dimension."""
+        if x.get_device() != self._dev:
             raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
-        if x.dtype not in (torch.float16, torch.bfloat16):
+        if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
             raise ValueError(f"{what} only supports fp16/bf16, got {x.dtype}")
-        if x.ndim != 4 or x.shape[0] != self.batch or x.shape[3] != self.head_dim \
-                or (heads is not None and x.shape[2] != heads):
+        s = x.shape
+        if len(s) != 4 or s[0] != self.batch or s[3] != self.head_dim or (heads is not None and s[2] != heads):
             raise ValueError(f"{name} must be [batch={self.batch}, t, {'heads' if heads is None else heads}, "
-                             f"head_dim={self.head_dim}], got {tuple(x.shape)}")
-        if like is not None and (x.shape != like.shape or x.dtype != like.dtype):
-            raise ValueError(f"Shape mismatch k={like.dtype} {tuple(like.shape)} v={x.dtype} {tuple(x.shape)}")
-        if x.stride(3) != 1:
-            x = x.contiguous()
-        s = x.stride()
-        return x, _Strides(s[0], s[1], s[2])
+                             f"head_dim={self.head_dim}], got {tuple(s)}")
+        return x if x.stride(3) == 1 else x.contiguous()
 
     def _lengths(self, lengths: torch.Tensor) -> int:
-        if lengths.device != self.device or lengths.dtype != torch.int32 or lengths.shape != (self.batch,) \
+        if lengths.get_device() != self._dev or lengths.dtype != torch.int32 or lengths.shape != (self.batch,) \
                 or not lengths.is_contiguous():
             raise ValueError(f"lengths must be a contiguous int32 tensor [{self.batch}] on {self.device}, got "
                              f"{lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
@@ -120,12 +117,15 @@ class KV4Cache:
         """Quantises k and v [batch, t, kv_heads, head_dim] (bf16 or fp16; any strides of the first
         three dimensions) into positions lengths[b] - t .. lengths[b] - 1; positions outside
         [0, max_seq_len) are skipped.  A group that holds an infinity or a NaN reads as NaN."""
-        k, ks = self._rows("KV4Cache.append", "k", k, self.num_kv_heads)
-        v, vs = self._rows("KV4Cache.append", "v", v, self.num_kv_heads, k)
+        k = self._rows("KV4Cache.append", "k", k, self.num_kv_heads)
+        v = self._rows("KV4Cache.append", "v", v, self.num_kv_heads)
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError(f"Shape mismatch k={k.dtype} {tuple(k.shape)} v={v.dtype} {tuple(v.shape)}")
         at = self._lengths(lengths)
-        no_grad("KV4Cache.append", k, v)
-        call(self._lib.mq_kv4_append, self._dev, self._ref, k.data_ptr(), ks, v.data_ptr(), vs, at,
-             k.shape[1], DTYPES[k.dtype])
+        if torch.is_grad_enabled():
+            no_grad("KV4Cache.append", k, v)
+        call(self._append, self._dev, self._ref, k.data_ptr(), _Strides(*k.stride()[:3]), v.data_ptr(),
+             _Strides(*v.stride()[:3]), at, k.shape[1], DTYPES[k.dtype])
 
     def read(self, lengths: torch.Tensor, t: int, dtype: torch.dtype = torch.bfloat16
              ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -138,10 +138,9 @@ class KV4Cache:
         if t < 0:
             raise ValueError(f"t must not be negative, got {t}")
         at = self._lengths(lengths)
-        shape = (self.batch, t, self.num_kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=self.device)
-        v = torch.empty(shape, dtype=dtype, device=self.device)
-        call(self._lib.mq_kv4_read, self._dev, self._ref, at, t, k.data_ptr(), v.data_ptr(), DTYPES[dtype])
+        k = self.scales.new_empty((self.batch, t, self.num_kv_heads, self.head_dim), dtype=dtype)
+        v = torch.empty_like(k)
+        call(self._read, self._dev, self._ref, at, t, k.data_ptr(), v.data_ptr(), DTYPES[dtype])
         return k, v
 
     def attend(self, q: torch.Tensor, lengths: torch.Tensor, *, scale: Optional[float] = None,
@@ -151,23 +150,24 @@ class KV4Cache:
         output has q's type and shape; a query with no position to look at gives 0.  `scale`
         defaults to 1/sqrt(head_dim).  max_length, if known, is an upper bound of `lengths`: the
         work is split for it, and positions from there on are not looked at."""
-        q, qs = self._rows("KV4Cache.attend", "q", q, None)
-        t, heads = q.shape[1], q.shape[2]
+        q = self._rows("KV4Cache.attend", "q", q, None)
+        _, t, heads, _ = q.shape
         if heads < 1 or heads % self.num_kv_heads != 0:
             raise ValueError(f"q has {heads} heads, not a multiple of {self.num_kv_heads}")
         at = self._lengths(lengths)
         n = self.max_seq_len if max_length is None else int(max_length)
         if not 0 <= n <= self.max_seq_len:
             raise ValueError(f"max_length {n} outside [0, max_seq_len={self.max_seq_len}]")
-        no_grad("KV4Cache.attend", q)
+        if torch.is_grad_enabled():
+            no_grad("KV4Cache.attend", q)
         if n == 0 or t == 0:
             return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
         # scratch of this call alone, in stream order: calls on other streams and captured graphs
         # have theirs
-        size = self._lib.mq_kv4_attend_workspace_bytes(self._ref, t, heads, n)
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        call(self._lib.mq_kv4_attend, self._dev, self._ref, q.data_ptr(), qs, at, t, heads, n,
+        size = self._workspace(self._ref, t, heads, n)
+        ws = self.k_codes.new_empty(size) if size else None
+        call(self._attend, self._dev, self._ref, q.data_ptr(), _Strides(*q.stride()[:3]), at, t, heads, n,
              DTYPES[q.dtype], scale, out.data_ptr(), None if ws is None else ws.data_ptr(), size)
         return out

@@ -36,39 +36,43 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top_k: int = 0
     most 32) most likely tokens; equal logits are ordered by the lower token.
     A row of -inf alone has no distribution: log probabilities -inf, entropy 0, tokens 0 ..
     top_k - 1.  A row that holds a NaN or +inf gives NaN."""
-    if logits.device.type != "cuda":
+    dtype, dev, shape = DTYPES.get(logits.dtype), logits.get_device(), logits.shape
+    if not logits.is_cuda:
         raise ValueError("token_logprobs expects CUDA tensors")
-    if logits.dtype not in DTYPES:
+    if dtype is None:
         raise ValueError(f"token_logprobs only supports fp16/bf16/fp32, got {logits.dtype}")
-    if logits.ndim < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be [..., vocab], got {tuple(logits.shape)}")
-    if tokens.device != logits.device:
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"logits must be [..., vocab], got {tuple(shape)}")
+    if tokens.get_device() != dev:
         raise ValueError(f"tokens is on {tokens.device}, logits on {logits.device}")
-    if tokens.dtype not in (torch.int32, torch.int64):
+    wide = tokens.dtype == torch.int64
+    if not wide and tokens.dtype != torch.int32:
         raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
-    lead, vocab, top_k = logits.shape[:-1], logits.shape[-1], int(top_k)
+    lead, vocab, top_k = (shape[0],) if len(shape) == 2 else tuple(shape[:-1]), shape[-1], int(top_k)
     if tokens.shape != lead:
-        raise ValueError(f"Shape mismatch logits={tuple(logits.shape)} tokens={tuple(tokens.shape)}")
-    if not 0 <= top_k <= min(MAX_TOP_K, vocab):
+        raise ValueError(f"Shape mismatch logits={tuple(shape)} tokens={tuple(tokens.shape)}")
+    if not 0 <= top_k <= MAX_TOP_K or top_k > vocab:
         raise ValueError(f"top_k must be in [0, min({MAX_TOP_K}, vocab={vocab})], got {top_k}")
-    no_grad("token_logprobs", logits)
-    if logits.ndim != 2:
+    if torch.is_grad_enabled():
+        no_grad("token_logprobs", logits)
+    if len(shape) != 2:
         logits = logits.reshape(-1, vocab)
-    if logits.stride(1) != 1 and vocab > 1:
+    stride, step = logits.stride()
+    if step != 1 and vocab > 1:
         logits = logits.contiguous()
+        stride = vocab
     tokens = tokens.contiguous()
-    rows, dev = logits.shape[0], logits.device
-    lp = torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    top_lp = torch.empty(lead + (top_k,), dtype=torch.float32, device=dev)
-    top_tok = torch.empty(lead + (top_k,), dtype=torch.int32, device=dev)
+    rows = logits.shape[0]
+    lp = logits.new_empty(lead, dtype=torch.float32)
+    entropy = torch.empty_like(lp)
+    top_lp = lp.new_empty((*lead, top_k))
+    top_tok = torch.empty_like(top_lp, dtype=torch.int32)
     if rows:
         lib = _lib.load()
         # scratch of this call alone, in stream order
         size = lib.mq_token_logprobs_workspace_bytes(rows, vocab, top_k)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        call(lib.mq_token_logprobs, logits.get_device(), logits.data_ptr(), logits.stride(0), tokens.data_ptr(),
-             tokens.dtype == torch.int64, lp.data_ptr(), entropy.data_ptr(), top_lp.data_ptr() or None,
-             top_tok.data_ptr() or None, rows, vocab, top_k, DTYPES[logits.dtype],
+        ws = lp.new_empty(size // 4) if size else None
+        call(lib.mq_token_logprobs, dev, logits.data_ptr(), stride, tokens.data_ptr(), wide, lp.data_ptr(),
+             entropy.data_ptr(), top_lp.data_ptr() or None, top_tok.data_ptr() or None, rows, vocab, top_k, dtype,
              None if ws is None else ws.data_ptr(), size)
     return TokenLogprobs(lp, entropy, top_lp, top_tok)

@@ -18,6 +18,7 @@ from . import _lib
 from ._launch import DTYPES, call, no_grad
 
 GROUP_SIZES = (32, 64, 128)
+_HALF = (torch.float16, torch.bfloat16)
 
 
 def quantize_w4(weight: torch.Tensor, group_size: int = 128, *, symmetric: bool = True,
@@ -60,12 +61,53 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     type, or fp32 with out_dtype=torch.float32 (logits); `residual` [..., N] of that type is added
     before its one rounding.  Sums are fp32.  Meant for up to about 64 rows of x (one pass over the
     weights per 64 rows); more rows are computed all the same."""
+    # (the checks are most of a short product's call: plain comparisons, the message in _refuse)
+    dtype, dev = x.dtype, x.get_device()
+    if not x.is_cuda or dtype not in _HALF or qweight.ndim != 2 or qweight.dtype != torch.uint8 \
+            or scales.ndim != 2 or scales.dtype not in _HALF:
+        _refuse(x, qweight, scales, zeros, residual, out_dtype)
+    (n, half), (sn, groups), shape = qweight.shape, scales.shape, x.shape
+    k = 2 * half
+    if not shape or shape[-1] != k or sn != n or groups < 1 or k % groups != 0 or k // groups not in GROUP_SIZES \
+            or qweight.get_device() != dev or scales.get_device() != dev \
+            or not (qweight.is_contiguous() and scales.is_contiguous()):
+        _refuse(x, qweight, scales, zeros, residual, out_dtype)
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape
+                              or zeros.get_device() != dev or not zeros.is_contiguous()):
+        _refuse(x, qweight, scales, zeros, residual, out_dtype)
+    if out_dtype is None:
+        out_dtype = dtype
+    elif out_dtype != dtype and out_dtype != torch.float32:
+        _refuse(x, qweight, scales, zeros, residual, out_dtype)
+    size = (shape[0], n) if len(shape) == 2 else (*shape[:-1], n)
+    if residual is not None and (residual.dtype != out_dtype or residual.shape != size or residual.get_device() != dev):
+        _refuse(x, qweight, scales, zeros, residual, out_dtype)
+    if torch.is_grad_enabled():
+        no_grad("w4_linear", x, scales, residual)
+    out = x.new_empty(size) if out_dtype == dtype else x.new_empty(size, dtype=out_dtype)
+    if out.numel() == 0:
+        return out
+    x = x.contiguous()
+    at = x.data_ptr()
+    if at % 16 != 0:
+        x = x.clone()
+        at = x.data_ptr()
+    if residual is not None:
+        residual = residual.contiguous()
+    call(_lib.load().mq_w4_linear, dev, at, qweight.data_ptr(), scales.data_ptr(),
+         None if zeros is None else zeros.data_ptr(),
+         None if residual is None else residual.data_ptr(), out.data_ptr(), x.numel() // k, n, k,
+         k // groups, DTYPES[dtype], DTYPES[scales.dtype], DTYPES[out_dtype])
+    return out
+
+
+def _refuse(x, qweight, scales, zeros, residual, out_dtype) -> None:
+    """Raises for the first of w4_linear's argument checks that fails."""
     if x.device.type != "cuda":
         raise ValueError("w4_linear expects CUDA tensors")
-    if x.dtype not in (torch.float16, torch.bfloat16):
+    if x.dtype not in _HALF:
         raise ValueError(f"w4_linear only supports fp16/bf16, got {x.dtype}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype != x.dtype and out_dtype != torch.float32:
+    if out_dtype not in (None, x.dtype, torch.float32):
         raise ValueError(f"out_dtype must be {x.dtype} or float32, got {out_dtype}")
     if qweight.ndim != 2 or qweight.dtype != torch.uint8:
         raise ValueError(f"qweight must be uint8 [N, K/2], got {qweight.dtype} {tuple(qweight.shape)}")
@@ -76,7 +118,7 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
             or k // scales.shape[1] not in GROUP_SIZES:
         raise ValueError(f"scales {tuple(scales.shape)} do not fit qweight {tuple(qweight.shape)} in "
                          f"groups of {GROUP_SIZES}")
-    if scales.dtype not in (torch.float16, torch.bfloat16):
+    if scales.dtype not in _HALF:
         raise ValueError(f"scales must be fp16/bf16, got {scales.dtype}")
     if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
         raise ValueError(f"zeros must be uint8 {tuple(scales.shape)}, got {zeros.dtype} {tuple(zeros.shape)}")
@@ -86,20 +128,5 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
                 raise ValueError(f"{name} is on {t.device}, x on {x.device}")
             if name != "residual" and not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
-    if residual is not None and (residual.dtype != out_dtype or residual.shape != x.shape[:-1] + (n,)):
-        raise ValueError(f"residual must be {out_dtype} {tuple(x.shape[:-1] + (n,))}, got "
-                         f"{residual.dtype} {tuple(residual.shape)}")
-    no_grad("w4_linear", x, scales, residual)
-    out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
-    if out.numel() == 0:
-        return out
-    x = x.contiguous()
-    if x.data_ptr() % 16 != 0:
-        x = x.clone()
-    if residual is not None:
-        residual = residual.contiguous()
-    call(_lib.load().mq_w4_linear, x.get_device(), x.data_ptr(), qweight.data_ptr(), scales.data_ptr(),
-         None if zeros is None else zeros.data_ptr(),
-         None if residual is None else residual.data_ptr(), out.data_ptr(), x.numel() // k, n, k,
-         k // scales.shape[1], DTYPES[x.dtype], DTYPES[scales.dtype], DTYPES[out_dtype])
-    return out
+    want = (x.dtype if out_dtype is None else out_dtype, (*x.shape[:-1], n))
+    raise ValueError(f"residual must be {want[0]} {want[1]}, got {residual.dtype} {tuple(residual.shape)}")
