@@ -67,13 +67,21 @@ MQ_DEV LpSum lp_join(LpSum a, LpSum b) {
   r.t = fa * fmaf(a.s, da, a.t) + fb * fmaf(b.s, db, b.t);
   return r;
 }
-// (the two lanes of a pair may round differently: every lane takes lane 0's)
+// Over the 64 lanes: the maximum first, then the sums at it.
+MQ_DEV float lp_wave_max(float v) {
+  v = lp_max(v, dpp_f<MQ_DPP_QUAD_XOR1>(v));
+  v = lp_max(v, dpp_f<MQ_DPP_QUAD_XOR2>(v));
+  v = lp_max(v, dpp_f<MQ_DPP_ROW_HALF_MIRROR>(v));
+  v = lp_max(v, dpp_f<MQ_DPP_ROW_MIRROR>(v));
+  float2 p = swap16(v);
+  p = swap32(lp_max(p.x, p.y));
+  return lp_max(p.x, p.y);
+}
+// (lane 0's in every lane: the order of a sum differs between lanes)
 MQ_DEV LpSum lp_wave_join(LpSum r) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1)
-    r = lp_join(r, LpSum{xor_lane(r.m, d), xor_lane(r.s, d), xor_lane(r.t, d)});
   auto first = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
-  return LpSum{first(r.m), first(r.s), first(r.t)};
+  const float m = first(lp_wave_max(r.m)), d = lp_y(r.m, m), f = __builtin_amdgcn_exp2f(d);
+  return LpSum{m, first(wave_sum(f * r.s)), first(wave_sum(f * fmaf(r.s, d, r.t)))};
 }
 // n more elements
 template <int N> MQ_DEV void lp_add(LpSum& r, const float (&x)[N]) {
@@ -100,7 +108,7 @@ MQ_DEV float lp_key_value(uint64_t k) {
 
 struct LpShared {
   LpSum sums[LP_WAVES];
-  float group[LP_GROUPS];
+  alignas(16) float group[LP_GROUPS];
   int n_gt, n_eq, n_scan;
   uint64_t best[LP_WAVES];
   uint16_t scan[LP_THREADS];
@@ -121,10 +129,18 @@ MQ_DEV LpRow lp_row(LpSum r) {
   w.ls = __builtin_amdgcn_logf(r.s) * LP_LN2;
   return w;
 }
-template <int TYPE> MQ_DEV void lp_write(const MqLogprobArgs& a, int row, LpSum r, const LpRow& w) {
+// The logit of a row's token, and whether it has one (loaded at a kernel's start, used at its end)
+struct LpToken {
+  float x;
+  bool in;
+};
+template <int TYPE> MQ_DEV LpToken lp_token(const MqLogprobArgs& a, int row) {
   const long long tok = a.tok64 ? ((const long long*)a.tokens)[row] : ((const int*)a.tokens)[row];
-  const auto* x = (const typename LpType<TYPE>::raw*)a.logits + (long long)row * a.stride;
-  a.logprob[row] = tok >= 0 && tok < a.vocab ? lp_of(w, lp_float<TYPE>(x[tok])) : w.bad ? NAN : -INFINITY;
+  const bool in = tok >= 0 && tok < a.vocab;
+  return LpToken{lp_float<TYPE>(((const typename LpType<TYPE>::raw*)a.logits)[(long long)row * a.stride + (in ? tok : 0)]), in};
+}
+MQ_DEV void lp_write(const MqLogprobArgs& a, int row, LpSum r, const LpRow& w, LpToken tok) {
+  a.logprob[row] = tok.in ? lp_of(w, tok.x) : w.bad ? NAN : -INFINITY;
   a.entropy[row] = w.bad ? NAN : w.empty ? 0.f : (__builtin_amdgcn_logf(r.s) - r.t / r.s) * LP_LN2;
 }
 
@@ -147,6 +163,8 @@ __global__ void __launch_bounds__(LP_THREADS) lp_slice_kernel(MqLogprobArgs a, i
   const int row = blockIdx.x / slices, sl = blockIdx.x - row * slices;
   const int lo = sl * slice, n = min(slice, a.vocab - lo);      // n >= 1
   const raw* x = (const raw*)a.logits + (long long)row * a.stride + lo;
+  LpToken tok = {};
+  if (slices == 1 && tid == 0) tok = lp_token<TYPE>(a, row);
 
   // Thread t has vectors t, t + 512, ..  and one of the last elements, or, in a slice too short to give
   // every thread a vector, elements t, t + 512, ..
@@ -188,12 +206,11 @@ __global__ void __launch_bounds__(LP_THREADS) lp_slice_kernel(MqLogprobArgs a, i
   if ((lane & 15) == 0) sh.group[tid >> 4] = gm;
   if (tid == 0) sh.n_gt = sh.n_eq = sh.n_scan = 0;
   __syncthreads();
-  r = sh.sums[0];
-#pragma unroll
-  for (int w = 1; w < LP_WAVES; ++w) r = lp_join(r, sh.sums[w]);
+  r = lane < LP_WAVES ? sh.sums[lane] : LpSum{-INFINITY, 0.f, 0.f};
+  r = lp_wave_join(r);
   const LpRow out = lp_row(r);
   if (tid == 0) {
-    if (slices == 1) lp_write<TYPE>(a, row, r, out);
+    if (slices == 1) lp_write(a, row, r, out, tok);
     else part_sum[blockIdx.x] = r;
   }
   const int k = a.top_k;
@@ -213,14 +230,17 @@ __global__ void __launch_bounds__(LP_THREADS) lp_slice_kernel(MqLogprobArgs a, i
     if (tid < kk) put(tid, lp_key(NAN, lo + tid));
     return;
   }
-  // B: the kk-th largest of the groups' maxima
-  const float g = sh.group[lane & (LP_GROUPS - 1)];
+  // B: the kk-th largest of the groups' maxima; lane l counts, of those larger than group l % 32's, the
+  // ones in one half of the groups
+  const int gi = lane & (LP_GROUPS - 1), g0 = (lane >> 5) * (LP_GROUPS / 2);
+  const float g = sh.group[gi];
   int above = 0;
 #pragma unroll
-  for (int i = 0; i < LP_GROUPS; ++i) {
-    const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), i));
-    above += o > g || (o == g && i < (lane & (LP_GROUPS - 1)));
+  for (int i = 0; i < LP_GROUPS / 2; ++i) {
+    const float o = sh.group[g0 + i];
+    above += o > g || (o == g && g0 + i < gi);
   }
+  above += __builtin_amdgcn_ds_bpermute((lane ^ 32) << 2, above);
   const uint64_t at = __builtin_amdgcn_ballot_w64(above == kk - 1);
   const float bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), __builtin_ctzll(at)));
   if (mine >= bound) sh.scan[atomicAdd(&sh.n_scan, 1)] = (uint16_t)tid;
@@ -234,24 +254,25 @@ __global__ void __launch_bounds__(LP_THREADS) lp_slice_kernel(MqLogprobArgs a, i
       if (c < LP_CAP) sh.eq[c] = lp_key(v, lo + i);
     }
   };
-  const int scans = sh.n_scan;
-  for (int c = wave; c < scans; c += LP_WAVES) {
-    const int t = sh.scan[c];
-    if (wide) {
-      for (int v = t + lane * LP_THREADS; v < nvec; v += 64 * LP_THREADS) {
-        float e[VEC];
-        lp_load<TYPE>(x + (size_t)v * VEC, e);
-        float mx = e[0];
+  // (thread, vector) pairs over the workgroup; a thread's last element counts as a vector
+  const int scans = sh.n_scan, full = wide ? (nvec + LP_THREADS - 1) / LP_THREADS : (n + LP_THREADS - 1) / LP_THREADS;
+  const int per = full + (rest > 0);
+  for (int id = tid; id < scans * per; id += LP_THREADS) {
+    const int c = id / per, q = id - c * per, t = sh.scan[c], v = t + q * LP_THREADS;
+    if (!wide) {
+      if (v < n) look(lp_float<TYPE>(x[v]), v);
+    } else if (q == full) {
+      if (t < rest) look(lp_float<TYPE>(x[nvec * VEC + t]), nvec * VEC + t);
+    } else if (v < nvec) {
+      float e[VEC];
+      lp_load<TYPE>(x + (size_t)v * VEC, e);
+      float mx = e[0];
 #pragma unroll
-        for (int i = 1; i < VEC; ++i) mx = fmaxf(mx, e[i]);
-        if (mx >= bound) {
+      for (int i = 1; i < VEC; ++i) mx = fmaxf(mx, e[i]);
+      if (mx >= bound) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) look(e[i], v * VEC + i);
-        }
+        for (int i = 0; i < VEC; ++i) look(e[i], v * VEC + i);
       }
-      if (lane == 0 && t < rest) look(lp_float<TYPE>(x[nvec * VEC + t]), nvec * VEC + t);
-    } else {
-      for (int i = t + lane * LP_THREADS; i < n; i += 64 * LP_THREADS) look(lp_float<TYPE>(x[i]), i);
     }
   }
   __syncthreads();
@@ -303,20 +324,28 @@ __global__ void __launch_bounds__(LP_THREADS) lp_slice_kernel(MqLogprobArgs a, i
 // j = ceil(k / slices), bound the k-th largest key from below by their ceil(k / j)-th largest.
 template <int TYPE>
 __global__ void __launch_bounds__(256) lp_join_kernel(MqLogprobArgs a, int slices, const LpSum* part_sum, const uint64_t* part_key) {
-  __shared__ uint64_t cand[LP_SLICES * MQ_TOP_MAX];
-  __shared__ uint64_t bound_sh;
+  constexpr int HELD = LP_SLICES * MQ_TOP_MAX / 256;
+  __shared__ uint64_t cand[LP_SLICES * MQ_TOP_MAX], lead[LP_SLICES];
   __shared__ int count;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, k = a.top_k;
+  const uint64_t* keys = part_key + (size_t)row * slices * k;
+  const int j = k > 0 ? (k + slices - 1) / slices : 1, need = (k + j - 1) / j, total = slices * k;      // need <= slices
+  // everything that is read, at once
+  LpToken tok = {};
+  if (tid == 0) tok = lp_token<TYPE>(a, row);
   LpSum r = {-INFINITY, 0.f, 0.f};
   if (lane < slices) r = part_sum[(size_t)row * slices + lane];
+  uint64_t mine = 0, held[HELD];
+  if (k > 0 && lane < slices) mine = keys[(size_t)lane * k + j - 1];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) held[i] = tid + 256 * i < total ? keys[tid + 256 * i] : 0;
   r = lp_wave_join(r);
   const LpRow out = lp_row(r);
   if (tid == 0) {
-    lp_write<TYPE>(a, row, r, out);
+    lp_write(a, row, r, out, tok);
     count = 0;
   }
   if (k == 0) return;
-  const uint64_t* keys = part_key + (size_t)row * slices * k;
   if (r.m != r.m) {
     if (tid < k) {
       a.top_tok[(size_t)row * k + tid] = tid;
@@ -324,23 +353,19 @@ __global__ void __launch_bounds__(256) lp_join_kernel(MqLogprobArgs a, int slice
     }
     return;
   }
-  if (tid < 64) {
-    const int j = (k + slices - 1) / slices, need = (k + j - 1) / j;      // need <= slices
-    const uint64_t mine = lane < slices ? keys[(size_t)lane * k + j - 1] : 0;
-    int above = 0;
-    for (int i = 0; i < slices; ++i) {
-      const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(mine >> 32), i), lo = __builtin_amdgcn_readlane((uint32_t)mine, i);
-      const uint64_t o = ((uint64_t)hi << 32) | lo;
-      above += o > mine || (o == mine && i < lane);
-    }
-    if (lane < slices && above == need - 1) bound_sh = mine;
-  }
+  if (tid < slices) lead[tid] = mine;
   __syncthreads();
-  const uint64_t bound = bound_sh;
-  for (int i = tid; i < slices * k; i += 256) {
-    const uint64_t key = keys[i];
-    if (key >= bound && key != 0) cand[atomicAdd(&count, 1)] = key;
+  // Every wave: the rank of each slice's j-th key (keys are different, but for 0: no key), and B
+  int above = 0;
+  for (int i = 0; i < slices; ++i) {
+    const uint64_t o = lead[i];
+    above += o > mine || (o == mine && i < lane);
   }
+  const uint64_t at = __builtin_amdgcn_ballot_w64(lane < slices && above == need - 1);
+  const uint64_t bound = lead[__builtin_ctzll(at)];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+    if (held[i] >= bound && held[i] != 0) cand[atomicAdd(&count, 1)] = held[i];
   __syncthreads();
   lp_rank(cand, count, k, [&](int i, uint64_t key) {
     a.top_tok[(size_t)row * k + i] = (int)argmax_key_index(key);
