@@ -330,7 +330,7 @@ int mq_kv4_read(const mq_kv4_cache* cache, const int32_t* d_lengths, int t, void
                 void* d_v_out, int out_dtype, void* stream);
 /* Attention over the cache: query row i of sequence b looks at positions 0 .. lengths[b] - t + i,
  *   out[b][i][h] = sum_p softmax_p(scale * q[b][i][h] . k[b][hk][p]) v[b][hk][p],
- * hk = h / (q_heads / kv_heads); a row that has no position to look at gives 0.  max_len bounds the
+ * hk = h / (q_heads / kv_heads), at most 256 kv heads with 256 query heads each; a row that has no position to look at gives 0.  max_len bounds the
  * positions that are looked at (lengths above it are cut to it) and decides how the work is split;
  * max_seq is always right.  d_q: [batch, t, q_heads, head_dim] of dtype with element strides
  * q_strides as above; out: contiguous, of the same type.  fp32 scores, softmax and sums.

@@ -783,6 +783,8 @@ int mq_kv4_read(const mq_kv4_cache* cache, const int32_t* d_lengths, int t, void
 static int check_attend(const mq_kv4_cache* c, int t, int q_heads, int max_len) {
   if (q_heads < 1 || q_heads % c->kv_heads != 0)
     return fail(MQ_ERR_INVALID_ARG, "q_heads %d is not a multiple of kv_heads %d", q_heads, c->kv_heads);
+  if (c->kv_heads > 256 || q_heads / c->kv_heads > 256)
+    return fail(MQ_ERR_INVALID_ARG, "more than 256 kv heads, or query heads per kv head (%d, %d)", c->kv_heads, q_heads);
   if (max_len < 1 || max_len > c->max_seq)
     return fail(MQ_ERR_INVALID_ARG, "max_len %d outside [1, max_seq=%d]", max_len, c->max_seq);
   if ((long long)t * q_heads > (1 << 24) || (long long)c->batch * t * q_heads > (1ll << 24))

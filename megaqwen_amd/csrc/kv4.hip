@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(MqKv4 c, void* k, void* v
 
 // ---- attention
 //
-// A workgroup is (sequence, kv head, a tile of its query rows, a range of positions); its 4 waves take
+// A workgroup is (sequence, kv head, a tile of its query rows, a share of the positions); its 4 waves take
 // 32 positions at a time and join their (max, sum, O) at the end.  Query rows of a kv head are
 // r = t (Hq / Hkv) + head, so that a cached row is read once for all of them.
 //   * S = K Q^T by 16 x 16 x 32 products of the codes (mq_nibble.h) and the unrounded queries.  A
@@ -105,7 +105,6 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(MqKv4 c, void* k, void* v
 //     rounding stays far below the output's; one bf16 would add an error of the output's own size.
 // Softmax statistics and sums are fp32.  Codes are 4 bytes (8 dims) per lane for values, so that a
 // lane sees 8 positions of the same dims without a transpose through LDS.
-#define AT_WAVES 4
 #define AT_TILE 32                 // positions per wave and step
 #define AT_RAISE 8.0f              // a column's reference point moves when a score exceeds it by 2^8
 #define AT_BIAS (NB_OFFSET + 8.0f)
@@ -117,9 +116,13 @@ struct AtArgs {
   uint16_t* out;
   float2* ml;                      // [rows][nsplit] (max, sum) and
   float* part;                     // [rows][nsplit][D] unnormalised sums, if nsplit > 1
-  int Hq, ratio, max_len, nsplit, row_tiles;
+  int Hq, ratio, max_len, nsplit;
+  uint32_t by_ratio, by_hkv;       // at_magic()
   float scale_log2;
 };
+// n / d as the upper half of n ceil(2^32 / d): exact for n (d - 1) < 2^32 (d <= 256 and n <= 2^24 here)
+uint32_t at_magic(int d) { return d == 1 ? 0u : (uint32_t)((0x100000000ull + d - 1) / d); }
+MQ_DEV int at_div(int n, uint32_t magic) { return magic == 0 ? n : (int)__umulhi((uint32_t)n, magic); }
 
 // 16 bits of a word as the upper half of an fp32 (a bf16 scale), chosen by a byte selector
 MQ_DEV float at_pick(uint32_t hi, uint32_t lo, uint32_t sel) { return __uint_as_float(__builtin_amdgcn_perm(hi, lo, sel)); }
@@ -148,91 +151,58 @@ MQ_DEV void at_split2(float w0, float w1, uint32_t& hi, uint32_t& lo) {
   lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2));
 }
 
-// 32 positions as a lane holds them: K words of position 16 t + col, dims (D / 4) j + ..; value dims
-// DPL col + .. and scales of positions 16 t + 4 j + i.
-template <int D, int NG> struct AtTile {
-  uint32_t k[2][D / 32], v[8], s[NG == 4 ? 16 : NG == 2 ? 16 : 8];
+// Scales of positions 16 t + 4 j + i of a tile, as a lane holds them
+template <int NG> struct AtScales {
+  uint32_t s[NG == 1 ? 8 : 16];
 };
 
-template <bool F16, int D, int NG, int CT>
-__global__ void __launch_bounds__(64 * AT_WAVES, CT == 1 ? 3 : 2) kv4_attend_kernel(AtArgs a) {
+template <bool F16, int D, int NG, int CT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, CT == 1 ? 4 : 2) kv4_attend_kernel(AtArgs a) {
   constexpr int KW = D / 32;       // words of a key row per lane
   constexpr int DPL = D / 16;      // dims of a value row per lane
   constexpr int RQ = 16 / NG;      // query rows per column tile
   constexpr int G = D / NG;
-  typedef AtTile<D, NG> Tile;
-  __shared__ float red[AT_WAVES][4 * DPL][64];
-  __shared__ float2 red_ml[AT_WAVES][CT][16];
+  typedef AtScales<NG> Scales;
+  __shared__ float red[WAVES][4 * DPL][64];
+  __shared__ float4 red_ml[WAVES][CT][16];       // m, l, and the sum that the offset is taken off by
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, j = lane >> 4, g = col % NG;
   // the kv head is the fastest index: workgroups go round the 8 XCDs, so that those that read the
   // same rows share an L2
-  int id = blockIdx.x;
-  const int hk = id % a.c.Hkv; id /= a.c.Hkv;
-  const int rt = id % a.row_tiles; id /= a.row_tiles;
-  const int split = id % a.nsplit, b = id / a.nsplit;
+  const int rt = at_div(blockIdx.x, a.by_hkv), hk = blockIdx.x - rt * a.c.Hkv, split = blockIdx.y, b = blockIdx.z;
   const int rows = a.c.T * a.ratio, r0 = rt * (CT * RQ);
   const int cap = min(a.c.S, a.max_len);
-  const long long first = (long long)a.c.lengths[b] - a.c.T + 1;      // positions of query t: first + t
-  auto limit = [&](int r) { return (int)max(0ll, min((long long)cap, first + r / a.ratio)); };
-  const int end = limit(min(r0 + CT * RQ, rows) - 1), sure = limit(r0);
-  const int chunk = ((end + a.nsplit - 1) / a.nsplit + AT_TILE - 1) / AT_TILE * AT_TILE;
-  const int p0 = split * chunk, p1 = min(end, p0 + chunk);
-  // scores are taken with the scale's sign in the queries, so that the largest stays the largest; a scale
-  // of 0 is one next to it, so that a masked score, -inf, stays -inf
-  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
-
-  uint4 qf[CT][KW];
-  // m: a column's reference point (lowest: none yet), l: its sum of weights in this lane's positions
-  float cinit[CT], m[CT], l[CT];
-  int lim[CT];
-  nb_f32x4 acc[CT][DPL], sv[CT];   // sv: the sums of the weights times the value scales, in every row
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int r = r0 + ct * RQ + col / NG;
-    const bool there = r < rows;
-    const int t = there ? r / a.ratio : 0, h = there ? hk * a.ratio + r % a.ratio : 0;
-    const uint16_t* qr = a.q + b * a.qs.b + t * a.qs.t + h * a.qs.h;
-    float sum = 0.f;
-#pragma unroll
-    for (int s = 0; s < KW; ++s) {
-      const int d = (D / 4) * j + 8 * s;
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (there && d / G == g) {
-        x = nb_order8(nb_load16(qr + d));
-        x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-      }
-      qf[ct][s] = x;
-      sum += nb_sum8<F16>(x);
-    }
-    cinit[ct] = -AT_BIAS * sum_xor32(sum_xor16(sum));
-    lim[ct] = there ? limit(r) : 0;
-    m[ct] = -3.402823466e38f;
-    l[ct] = 0.f;
-    sv[ct] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) acc[ct][i] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  // rows of this (sequence, kv head): loads beyond its last row in sight return 0 without an access
+  // rows of this (sequence, kv head): loads beyond its last row return 0 without an access
   const size_t row = ((size_t)b * a.c.Hkv + hk) * a.c.S;
   auto rsrc = [&](const void* base, int row_bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + row * row_bytes), (short)0, end * row_bytes, 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + row * row_bytes), (short)0, cap * row_bytes, 0x00020000);
   };
   const __amdgpu_buffer_rsrc_t kr = rsrc(a.c.kq, D / 2), vr = rsrc(a.c.vq, D / 2), sr = rsrc(a.c.scales, 4 * NG);
-  auto load = [&](Tile& x, int p) {
+  // A tile: K words of position 16 t + col, dims (D / 4) j + ..; value dims DPL col + .. of positions
+  // 16 t + 4 j + i.  The next tile's words are loaded over a tile's as soon as those are used.
+  uint32_t kw[2][KW], vw[8];
+  auto load_keys = [&](int p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int ko = (p + 16 * t + col) * (D / 2) + j * (4 * KW);
       if constexpr (KW == 4) {
         const auto w = __builtin_amdgcn_raw_buffer_load_b128(kr, ko, 0, 0);
-        for (int s = 0; s < 4; ++s) x.k[t][s] = w[s];
+        for (int s = 0; s < 4; ++s) kw[t][s] = w[s];
       } else {
         const auto w = __builtin_amdgcn_raw_buffer_load_b64(kr, ko, 0, 0);
-        for (int s = 0; s < 2; ++s) x.k[t][s] = w[s];
+        for (int s = 0; s < 2; ++s) kw[t][s] = w[s];
       }
     }
+  };
+  auto load_values = [&](int p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int pos = p + 16 * (e >> 2) + 4 * j + (e & 3);
+      if constexpr (DPL == 8) vw[e] = __builtin_amdgcn_raw_buffer_load_b32(vr, pos * (D / 2) + 4 * col, 0, 0);
+      else vw[e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vr, pos * (D / 2) + 2 * col, 0, 0);
+    }
+  };
+  auto load_scales = [&](Scales& x, int p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if constexpr (NG == 1) {           // (key, value) scale pairs of 4 positions
@@ -250,34 +220,87 @@ __global__ void __launch_bounds__(64 * AT_WAVES, CT == 1 ? 3 : 2) kv4_attend_ker
           x.s[2 * e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * 16 + 2 * g, 0, 0);
           x.s[2 * e + 1] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * 16 + 8 + 2 * g, 0, 0);
         }
-        if constexpr (DPL == 8) x.v[e] = __builtin_amdgcn_raw_buffer_load_b32(vr, pos * (D / 2) + 4 * col, 0, 0);
-        else x.v[e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vr, pos * (D / 2) + 2 * col, 0, 0);
       }
     }
   };
+  // positions that query t looks at: first + t, in [0, cap]
+  const int first = min(max(a.c.lengths[b], 0), 1 << 28) - a.c.T + 1;
+  auto limit = [&](int r) { return max(0, min(cap, first + at_div(r, a.by_ratio))); };
+  const int end = limit(min(r0 + CT * RQ, rows) - 1), sure = limit(r0);
+  // A range is contiguous (ranges dealt out tile by tile read 15% slower); without ranges a wave's first
+  // tile does not depend on the length.
+  constexpr int STRIDE = AT_TILE * WAVES;
+  int p = AT_TILE * wave, p1 = end;
+  if (a.nsplit > 1) {
+    const int chunk = ((end + a.nsplit - 1) / a.nsplit + STRIDE - 1) / STRIDE * STRIDE;
+    p += split * chunk;
+    p1 = min(end, (split + 1) * chunk);
+  }
+  Scales sx, sy;
+  load_keys(p);
+  load_scales(sx, p);
+  load_values(p);
+  // scores are taken with the scale's sign in the queries, so that the largest stays the largest; a scale
+  // of 0 is one next to it, so that a masked score, -inf, stays -inf
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
+
+  uint4 qf[CT][KW];
+  // m: a column's reference point (lowest: none yet), l: its sum of weights in this lane's positions
+  float m[CT], l[CT];
+  int lim[CT];
+  nb_f32x4 acc[CT][DPL], sv[CT];   // sv: the sums of the weights times the value scales, in every row
+  nb_f32x4 cinit[CT];              // -24 times the sum of the column's queries: the codes' offset
+  constexpr uint32_t BIAS2 = F16 ? 0xce00ce00u : 0xc1c0c1c0u;         // (-24, -24)
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int r = r0 + ct * RQ + col / NG;
+    const bool there = r < rows;
+    const int t = there ? at_div(r, a.by_ratio) : 0, h = there ? hk * a.ratio + r - t * a.ratio : 0;
+    const uint16_t* qr = a.q + b * a.qs.b + t * a.qs.t + h * a.qs.h;
+    cinit[ct] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KW; ++s) {
+      const int d = (D / 4) * j + 8 * s;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (there && d / G == g) {
+        x = nb_order8(nb_load16(qr + d));
+        x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+      }
+      qf[ct][s] = x;
+      cinit[ct] = nb_mfma<F16>(make_uint4(BIAS2, BIAS2, BIAS2, BIAS2), x, cinit[ct]);
+    }
+    lim[ct] = there ? limit(r) : 0;
+    m[ct] = -3.402823466e38f;
+    l[ct] = 0.f;
+    sv[ct] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[ct][i] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
   const uint32_t half = NG == 2 && g == 1 ? 0x03020c0cu : 0x01000c0cu;      // (0x0c: a zero byte)
-  auto key_scale = [&](const Tile& x, int e) {
+  auto key_scale = [&](const Scales& x, int e) {
     if constexpr (NG == 1) return __uint_as_float(x.s[e] << 16);
     else if constexpr (NG == 2) return at_pick(x.s[2 * e], x.s[2 * e], half);
     else return __uint_as_float(x.s[2 * e] << 16);
   };
-  auto value_scale = [&](const Tile& x, int e) {
+  auto value_scale = [&](const Scales& x, int e) {
     if constexpr (NG == 1) return __uint_as_float(x.s[e] & 0xffff0000u);
     else if constexpr (NG == 2) return at_pick(x.s[2 * e + 1], x.s[2 * e + 1], half);
     else return __uint_as_float(x.s[2 * e + 1] << 16);
   };
 
-  auto step = [&](const Tile& x, int p) {
+  auto step = [&](const Scales& x, Scales& next, int p) {
     // scores z[ct][e], not yet scaled, of positions p + 16 (e / 4) + 4 j + e % 4
     float z[CT][8];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       nb_f32x4 s[CT];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) s[ct] = nb_f32x4{cinit[ct], cinit[ct], cinit[ct], cinit[ct]};
+      for (int ct = 0; ct < CT; ++ct) s[ct] = cinit[ct];
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const uint4 kx = nb_expand8<F16>(x.k[t][w]);
+        const uint4 kx = nb_expand8<F16>(kw[t][w]);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) s[ct] = nb_mfma<F16>(kx, qf[ct][w], s[ct]);
       }
@@ -293,6 +316,8 @@ __global__ void __launch_bounds__(64 * AT_WAVES, CT == 1 ? 3 : 2) kv4_attend_ker
         }
       }
     }
+    load_keys(p + STRIDE);               // (past the end: not used)
+    load_scales(next, p + STRIDE);
     if (p + AT_TILE > sure) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
@@ -341,9 +366,10 @@ __global__ void __launch_bounds__(64 * AT_WAVES, CT == 1 ? 3 : 2) kv4_attend_ker
     uint32_t wl[4], wh[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      wl[t] = __builtin_amdgcn_perm(x.v[2 * t + 1], x.v[2 * t], 0x05040100u);
-      if constexpr (DPL == 8) wh[t] = __builtin_amdgcn_perm(x.v[2 * t + 1], x.v[2 * t], 0x07060302u);
+      wl[t] = __builtin_amdgcn_perm(vw[2 * t + 1], vw[2 * t], 0x05040100u);
+      if constexpr (DPL == 8) wh[t] = __builtin_amdgcn_perm(vw[2 * t + 1], vw[2 * t], 0x07060302u);
     }
+    load_values(p + STRIDE);
     auto values = [&](auto f_tag, const uint32_t (&w)[4], int i) {
       constexpr int f = decltype(f_tag)::value;
       const uint4 va = make_uint4(nb_pair<false, f>(w[0]), nb_pair<false, f>(w[1]), nb_pair<false, f>(w[2]), nb_pair<false, f>(w[3]));
@@ -364,16 +390,10 @@ __global__ void __launch_bounds__(64 * AT_WAVES, CT == 1 ? 3 : 2) kv4_attend_ker
       values(std::integral_constant<int, 3>(), wh, 7);
     }
   };
-  constexpr int STRIDE = AT_TILE * AT_WAVES;
-  Tile x, y;
-  int p = p0 + AT_TILE * wave;
-  if (p < p1) load(x, p);
-  for (; p < p1; p += 2 * STRIDE) {          // (loads past the end: zeros, not used)
-    load(y, p + STRIDE);
-    step(x, p);
+  for (; p < p1; p += 2 * STRIDE) {
+    step(sx, sy, p);
     if (p + STRIDE >= p1) break;
-    load(x, p + 2 * STRIDE);
-    step(y, p + STRIDE);
+    step(sy, sx, p + STRIDE);
   }
 
   // Join the waves.  A column's O, without the codes' offset, is in value order i' DPL + i, where
@@ -381,7 +401,7 @@ __global__ void __launch_bounds__(64 * AT_WAVES, CT == 1 ? 3 : 2) kv4_attend_ker
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     l[ct] = sum_xor32(sum_xor16(l[ct]));
-    if (j == 0) red_ml[wave][ct][col] = make_float2(m[ct], l[ct]);
+    if (j == 0) red_ml[wave][ct][col] = make_float4(m[ct], l[ct], sv[ct][0], 0.f);
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -389,28 +409,33 @@ __global__ void __launch_bounds__(64 * AT_WAVES, CT == 1 ? 3 : 2) kv4_attend_ker
 #pragma unroll
     for (int i = 0; i < DPL; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[wave][e * DPL + i][lane] = fmaf(-AT_BIAS, sv[ct][e], acc[ct][i][e]);
+      for (int e = 0; e < 4; ++e) red[wave][e * DPL + i][lane] = acc[ct][i][e];
     __syncthreads();
-    float mx = -INFINITY, sum = 0.f, f[AT_WAVES];
+    if (wave >= 4) continue;
+    float mx = -INFINITY, sum = 0.f, off = 0.f, f[WAVES];
+    float4 v[WAVES];
 #pragma unroll
-    for (int w = 0; w < AT_WAVES; ++w) mx = fmaxf(mx, red_ml[w][ct][col].x);
+    for (int w = 0; w < WAVES; ++w) v[w] = red_ml[w][ct][col];
 #pragma unroll
-    for (int w = 0; w < AT_WAVES; ++w) {
-      const float2 v = red_ml[w][ct][col];
-      f[w] = v.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v.x - mx);
-      sum = fmaf(v.y, f[w], sum);
+    for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, v[w].x);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {      // (a wave without a position: sums of 0 at the lowest m)
+      f[w] = __builtin_amdgcn_exp2f(v[w].x - mx);
+      sum = fmaf(v[w].y, f[w], sum);
+      off = fmaf(v[w].z, f[w], off);
     }
     // wave i' of the workgroup: dims DPL (4 j + i') .. + DPL of the lane's column
     float o[DPL];
 #pragma unroll
     for (int i = 0; i < DPL; ++i) {
-      o[i] = 0.f;
+      o[i] = -AT_BIAS * off;
 #pragma unroll
-      for (int w = 0; w < AT_WAVES; ++w) o[i] = f[w] == 0.f ? o[i] : fmaf(red[w][wave * DPL + i][lane], f[w], o[i]);
+      for (int w = 0; w < WAVES; ++w) o[i] = fmaf(red[w][wave * DPL + i][lane], f[w], o[i]);
     }
     const int r = r0 + ct * RQ + col / NG, d = DPL * (4 * j + wave);
     if (r >= rows || d / G != g) continue;
-    const size_t at = ((size_t)b * a.c.T + r / a.ratio) * a.Hq + hk * a.ratio + r % a.ratio;
+    const int t = at_div(r, a.by_ratio);
+    const size_t at = ((size_t)b * a.c.T + t) * a.Hq + hk * a.ratio + r - t * a.ratio;
     if (a.nsplit == 1) {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
       uint32_t w[DPL / 2];
@@ -483,7 +508,22 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const float2* ml, const f
   ((uint2*)out)[at * DT + d] = make_uint2(lo, hi);
 }
 
-// How a call is laid out: column tiles per workgroup and ranges of positions.
+// How a call is laid out.  Measured on 8 kv heads of 128 dims, bf16 and fp16:
+//  - query rows: one column tile if they fit, else two tiles per step, so that a tile's codes are
+//    read out of the registers twice (509 queries over 6007 rows: one tile 55 us, two 45 us).
+//  - waves: a workgroup's waves go through its positions in turns of 32.  Two column tiles take 8
+//    waves (4: 51 us for the 45 above), one tile 4 (a batch of 24 ragged sequences up to 8191 rows,
+//    4 query heads per kv head: 33.8 us, 8 waves 36.6 at their best; one sequence of 32768 rows 15.4
+//    and 14.8).
+//  - ranges: every workgroup costs about 2 us besides its positions, so one sequence gets as many as
+//    fill the 256 CUs once (32768 rows: 256 workgroups 15.4 us, 512 15.6, 1024 19.6; the 509
+//    queries: 256 45 us, 512 58).  Sequences in a batch differ in length and their workgroups with
+//    them; more per CU even that out: four of one tile (256 43 us, 512 40, 1024 34, 1536 36), two of
+//    two tiles (24 sequences of 4 query rows of 4 heads: 256 56 us, 512 53, 1024 66; of 2 rows of 2
+//    heads in groups of 32: 41, 36, 32; 5 sequences of 16 rows of 2 heads: 30, 34, 43).
+//    No range is shorter than AT_RANGE positions, and up to twice that one workgroup takes them all:
+//    the join is a kernel more.
+constexpr int AT_RANGE = 256;
 struct AtPlan {
   int ct, row_tiles, nsplit;
 };
@@ -492,10 +532,9 @@ AtPlan at_plan(int B, int T, int Hq, int Hkv, int D, int G, int max_len) {
   const int rq = 16 / (D / G), rows = T * (Hq / Hkv);
   p.ct = rows <= rq ? 1 : 2;
   p.row_tiles = (rows + p.ct * rq - 1) / (p.ct * rq);
-  const long long wgs = (long long)B * Hkv * p.row_tiles;
-  const int most = max_len <= 512 ? 1 : (max_len + 255) / 256;
-  const long long want = (512 + wgs - 1) / wgs;
-  p.nsplit = (int)(want < most ? want : most);
+  const long long wgs = (long long)B * Hkv * p.row_tiles, fill = B == 1 ? 256 : p.ct == 2 ? 512 : 1024;
+  const int want = (int)((fill + wgs - 1) / wgs), most = max_len <= 2 * AT_RANGE ? 1 : (max_len + AT_RANGE - 1) / AT_RANGE;
+  p.nsplit = want < most ? want : most;
   return p;
 }
 
@@ -542,13 +581,13 @@ int mq_launch_kv4_attend(const MqKv4& c, const uint16_t* q, MqStrides qs, uint16
   const AtPlan p = at_plan(c.B, c.T, Hq, c.Hkv, c.D, c.G, max_len);
   const size_t rows = (size_t)c.B * c.T * Hq;
   AtArgs a = {c, q, qs, out, (float2*)ws, (float*)((char*)ws + (rows * p.nsplit * sizeof(float2) + 15) / 16 * 16),
-              Hq, Hq / c.Hkv, max_len, p.nsplit, p.row_tiles, scale_log2};
-  const dim3 grid((unsigned)((long long)c.B * c.Hkv * p.row_tiles * p.nsplit)), block(64 * AT_WAVES);
+              Hq, Hq / c.Hkv, max_len, p.nsplit, at_magic(Hq / c.Hkv), at_magic(c.Hkv), scale_log2};
+  const dim3 grid((unsigned)(c.Hkv * p.row_tiles), (unsigned)p.nsplit, (unsigned)c.B), block(p.ct == 2 ? 512 : 256);
   auto go = [&](auto f16_, auto d, auto ng) {
     constexpr bool F = decltype(f16_)::value;
     constexpr int D = decltype(d)::value, NG = decltype(ng)::value;
-    if (p.ct == 1) hipLaunchKernelGGL((kv4_attend_kernel<F, D, NG, 1>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((kv4_attend_kernel<F, D, NG, 2>), grid, block, 0, stream, a);
+    if (p.ct == 2) hipLaunchKernelGGL((kv4_attend_kernel<F, D, NG, 2, 8>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((kv4_attend_kernel<F, D, NG, 1, 4>), grid, block, 0, stream, a);
     if (p.nsplit >= 16)
       hipLaunchKernelGGL((kv4_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a.ml, a.part, out, (int)rows, p.nsplit, F);
     else if (p.nsplit > 1)

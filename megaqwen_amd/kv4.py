@@ -146,7 +146,7 @@ class KV4Cache:
     def attend(self, q: torch.Tensor, lengths: torch.Tensor, *, scale: Optional[float] = None,
                max_length: Optional[int] = None) -> torch.Tensor:
         """Causal attention of q [batch, t, q_heads, head_dim] (bf16 or fp16, q_heads a multiple of
-        kv_heads) over the cache: query i of t looks at positions 0 .. lengths[b] - t + i.  The
+        kv_heads, neither kv heads nor query heads per kv head above 256) over the cache: query i of t looks at positions 0 .. lengths[b] - t + i.  The
         output has q's type and shape; a query with no position to look at gives 0.  `scale`
         defaults to 1/sqrt(head_dim).  max_length, if known, is an upper bound of `lengths`: the
         work is split for it, and positions from there on are not looked at."""

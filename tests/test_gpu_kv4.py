@@ -322,3 +322,13 @@ def test_argument_contracts():
     k = k.detach()
     assert c.attend(k[:, :0], n).shape == (2, 0, 4, 128) and c.read(n, 0)[0].shape == (2, 0, 4, 128)
     c.append(k[:, :0], k[:, :0], n)
+
+
+@pytest.mark.parametrize("b,t,h,r,s", [(2, 5, 7, 3, 700), (1, 3, 1, 256, 40), (1, 1, 256, 2, 33), (3, 11, 5, 13, 90),
+                                       (1, 2, 3, 255, 1100)])
+def test_attend_odd_and_largest_head_counts(b, t, h, r, s):
+    """Every query row finds its head and its position for head counts that are no power of two."""
+    c = _cache(b, h, s, 128, 64)
+    _fill(c, seed=31)
+    q, lens = _randn((b, t, h * r, 128), 32), [s - 5 * i for i in range(b)]
+    _check_attend(c, q, lens, c.attend(q, _lengths(lens)))

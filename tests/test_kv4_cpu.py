@@ -86,3 +86,14 @@ def test_c_abi_rejections():
         assert att(desc(b=1, n=32768), ml=32768, ws=None) == bad
     assert lib.mq_kv4_attend_workspace_bytes(None, 1, 8, 100) == 0
     assert lib.mq_kv4_attend_workspace_bytes(desc(), 1, 7, 100) == 0
+
+
+def test_c_abi_attend_head_limits():
+    lib, A = _lib.load(), 1 << 24
+    st = (ctypes.c_int64 * 3)(1 << 20, 1 << 20, 128)
+    for h, hq in ((1, 257), (257, 257), (2, 514), (300, 600)):
+        c = ctypes.byref(_lib.Kv4Cache(A, 2 * A, 3 * A, 1, h, 100, 128, 32))
+        assert lib.mq_kv4_attend(c, 4 * A, st, 6 * A, 1, hq, 100, _lib.MQ_DTYPE_BF16, 0.1, 5 * A, 7 * A, A,
+                                 None) == _lib.MQ_ERR_INVALID_ARG
+        assert b"256" in lib.mq_last_error()
+        assert lib.mq_kv4_attend_workspace_bytes(c, 1, hq, 100) == 0
