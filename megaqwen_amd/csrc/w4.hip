@@ -14,11 +14,11 @@
 // instruction per word or half of one), which keeps the 16-byte loads.
 //
 // Three kernels, by the sizes (w4_plan()):
-//   w4_direct_kernel   few outputs and up to 16 rows: the 8 waves of a workgroup split the inputs of 16
-//                      outputs and load their own pieces of x; nothing waits before the first product
+//   w4_direct_kernel   few outputs: the 8 waves of a workgroup split the inputs of 16 outputs and 16 rows
+//                      and load their own pieces of x; nothing waits before the first product
 //   w4_whole_kernel    several tiles of 16 outputs per workgroup share the rows of x, which wait in LDS in
 //                      operand order; kw waves split a tile's inputs
-//   w4_stretch_kernel  the same where the rows do not fit: a stretch of inputs after the other, two in LDS
+//   w4_stretch_kernel  the same where the rows do not fit: 512 inputs after the other, two such in LDS
 // x through LDS also keeps the loads of weights ahead of their use: loads return in order, so one of x
 // behind them would wait for memory.
 #include <hip/hip_runtime.h>
@@ -98,7 +98,7 @@ template <int G, int U> struct W4Weights {
     j = lane >> 4;
     wide = wide_scales;
     zeros = a.zeros != nullptr;
-    const int rows = max(0, min(16, a.N - n0));
+    const int rows = __builtin_amdgcn_readfirstlane(max(0, min(16, a.N - n0)));   // (resources stay in scalar registers)
     wr = rsrc(a.qw, K / 2, n0, rows);
     sr = rsrc(a.scales, groups * 2, n0, rows);
     zr = rsrc(a.zeros, groups, n0, rows);
@@ -157,18 +157,22 @@ template <int G, int U> struct W4Weights {
 // acc[t] += the products of a block whose first group is the first-th of sc (s16: all ones if the scales are
 // fp16, 0 for bf16); x_of(t, step) is the operand of row tile t.  A step's operands are read one step ahead, and no further: steps mixed by the scheduler
 // take more registers than there are.
-template <bool F16, int G, int MT, bool ONE, int NS, class X>
+template <bool F16, int G, int MT, bool ONE, bool AHEAD = true, int NS, class X>
 MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& sc, int first, uint32_t s16, X x_of) {
   constexpr int SPG = G / 32;            // steps of a group
   w4_exchange<G>(d);
   uint4 x[MT], zero;
   nb_f32x4 c[MT];
+  if constexpr (AHEAD)
 #pragma unroll
-  for (int t = 0; t < MT; ++t) x[t] = x_of(t, 0);
+    for (int t = 0; t < MT; ++t) x[t] = x_of(t, 0);
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     uint4 xn[MT];
-    if (s < 3) {
+    if constexpr (!AHEAD) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) x[t] = x_of(t, s);
+    } else if (s < 3) {
 #pragma unroll
       for (int t = 0; t < MT; ++t) xn[t] = x_of(t, s + 1);
     }
@@ -198,8 +202,9 @@ MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& 
       for (int t = 0; t < MT; ++t) asm volatile("" : "+v"(acc[t]));      // (here, and not behind the next loads)
     }
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (AHEAD)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) x[t] = xn[t];
+      for (int t = 0; t < MT; ++t) x[t] = xn[t];
   }
 }
 
@@ -236,7 +241,7 @@ MQ_DEV void w4_finish(const MqW4Args& a, const nb_f32x4 (&acc)[MT], int m0, int 
   }
 }
 
-// Up to 16 rows; wave w takes blocks w, w + 8, .. of the workgroup's 16 outputs.
+// 16 rows; wave w takes blocks w, w + 8, .. of the workgroup's 16 outputs.
 template <bool F16, int G, bool ONE>
 __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bool wide_scales) {
   constexpr int U = 3;                  // blocks in flight, with their pieces of x
@@ -245,8 +250,9 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
   const int lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4, blocks = (a.K + 127) / 128;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Weights wt(a, blockIdx.x * 16, wide_scales, lane);
-  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, (short)0, a.M * a.K * 2, 0x00020000);
-  const int xrow = (ONE ? 0 : min(col, a.M - 1)) * a.K;      // (rows past the last read it again)
+  const int m0 = 16 * blockIdx.y, rows = min(16, a.M - m0);
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (size_t)m0 * a.K), (short)0, rows * a.K * 2, 0x00020000);
+  const int xrow = (ONE ? 0 : min(col, rows - 1)) * a.K;     // (rows past the last read it again)
   struct Stretch {
     uint32_t w[4];
     W4Scales<Weights::NS> sc;
@@ -276,7 +282,7 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
       if (b + W4_WAVES * (u + U) < blocks) load(y[u], b + W4_WAVES * (u + U));
     }
   }
-  w4_finish<1, ONE>(a, acc, 0, a.M, wave, W4_WAVES, red);
+  w4_finish<1, ONE>(a, acc, m0, rows, wave, W4_WAVES, red);
 }
 
 struct W4Plan {
@@ -290,34 +296,32 @@ struct W4Plan {
 
 // Rows of x in LDS, in operand order: [rows][block][step][j][8], rows 16 bytes further apart than their
 // length, so that they start in different banks.
-template <int G, bool POW2> struct W4Rows {
+template <int G> struct W4Rows {
   const uint16_t* x;
-  int K, rows, per_row, stride;          // 16-byte pieces of a row (POW2: a power of two); elements
-  int shift;
+  int K, rows, per_row, stride;          // 16-byte pieces of a row; elements
   MQ_DEV W4Rows(const MqW4Args& a, int m0, int rows_, int blocks) {
     x = a.x + (size_t)m0 * a.K;
     K = a.K;
     rows = rows_;
     per_row = 16 * blocks;
-    shift = 31 - __builtin_clz(per_row);
     stride = 128 * blocks + 8;
   }
-  // piece `id` of the stretch of inputs that starts at block c0, zeros from K on
-  MQ_DEV uint4 fetch(int id, int c0) const {
-    const int m = POW2 ? id >> shift : id / per_row, k = c0 * 128 + 8 * (id - m * per_row);
+  // piece `id`, zeros from K on
+  MQ_DEV uint4 fetch(int id) const {
+    const int m = id / per_row, k = 8 * (id - m * per_row);
     return k < K ? ld16(x + (size_t)m * K + k) : make_uint4(0u, 0u, 0u, 0u);
   }
   MQ_DEV void put(uint16_t* dst, int id, uint4 v) const {
-    const int m = POW2 ? id >> shift : id / per_row, q = id - m * per_row;
+    const int m = id / per_row, q = id - m * per_row;
     *(uint4*)(dst + (size_t)m * stride + (q >> 4) * 128 + 8 * w4_slot<G>(q & 15)) = nb_order8(v);
   }
-  MQ_DEV void all(uint16_t* dst, int c0) const {
+  MQ_DEV void all(uint16_t* dst) const {
     const int total = rows * per_row, threads = blockDim.x;
     for (int id = threadIdx.x; id < total; id += 4 * threads) {
       uint4 v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (id + i * threads < total) v[i] = fetch(id + i * threads, c0);
+        if (id + i * threads < total) v[i] = fetch(id + i * threads);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (id + i * threads < total) put(dst, id + i * threads, v[i]);
@@ -326,8 +330,10 @@ template <int G, bool POW2> struct W4Rows {
 };
 
 #define W4_WHOLE_UNIT 4      // blocks of 128 inputs that a wave has in flight
-#define W4_STRETCH_UNIT 2    // blocks per wave and stretch; twice as many in flight
-#define W4_PIECES 8          // 16-byte pieces of x that a thread carries from one stretch to the next
+#define W4_STRETCH_KW 4      // waves that split the inputs, and blocks of a stretch
+#define W4_STRETCH_TILES 4   // tiles of 16 outputs
+#define W4_STRETCH_WAVES (W4_STRETCH_KW * W4_STRETCH_TILES)
+#define W4_STRETCH_ROW (128 * W4_STRETCH_KW + 8)
 
 template <bool F16, int G, int MT, bool ONE>
 __global__ void __launch_bounds__(W4_THREADS, MT == 2 ? 2 : G == 32 && !ONE ? 3 : 4) w4_whole_kernel(MqW4Args a, W4Plan pl) {
@@ -345,8 +351,8 @@ __global__ void __launch_bounds__(W4_THREADS, MT == 2 ? 2 : G == 32 && !ONE ? 3 
 #pragma unroll
   for (int u = 0; u < U; ++u) wt.codes(w[u], kw * U + u);
   wt.scales(sc, kw);
-  const W4Rows<G, false> rx(a, m0, rows, pl.units * U * pl.kw);
-  rx.all(xs, 0);
+  const W4Rows<G> rx(a, m0, rows, pl.units * U * pl.kw);
+  rx.all(xs);
   nb_f32x4 acc[MT];
   int xrow[MT];                          // (rows past the last read it again; their results are not stored)
 #pragma unroll
@@ -374,98 +380,101 @@ __global__ void __launch_bounds__(W4_THREADS, MT == 2 ? 2 : G == 32 && !ONE ? 3 
 }
 
 template <bool F16, int G, int MT>
-__global__ void __launch_bounds__(W4_THREADS, MT == 1 ? 3 : 2) w4_stretch_kernel(MqW4Args a, W4Plan pl) {
-  constexpr int U = W4_STRETCH_UNIT;
-  typedef W4Weights<G, U> Weights;
+__global__ void __launch_bounds__(64 * W4_STRETCH_WAVES, 4) w4_stretch_kernel(MqW4Args a, bool wide_scales) {
+  typedef W4Weights<G, 1> Weights;
+  constexpr int HALF = 16 * MT * W4_STRETCH_ROW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
+  uint16_t* xs = (uint16_t*)lds;                       // [2] stretches of [16 MT] rows
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = wave / pl.kw, kw = wave - nw * pl.kw;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = wave / W4_STRETCH_KW, kw = wave % W4_STRETCH_KW;
   const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
-  const Weights wt(a, (blockIdx.x * (W4_WAVES / pl.kw) + nw) * 16, pl.wide_scales, lane);
+  const Weights wt(a, (blockIdx.x * W4_STRETCH_TILES + nw) * 16, wide_scales, lane);
   const uint32_t s16 = a.s_type == MQ_T_F16 ? ~0u : 0u;
-  const int sblocks = U * pl.kw;                       // blocks of a stretch
-  const W4Rows<G, true> rx(a, m0, rows, sblocks);
-  uint16_t* xs = (uint16_t*)lds;                       // [2] stretches
-  const int half = rows * rx.stride, total = rows * rx.per_row;
-  // weights of this stretch and the next
-  uint32_t w[2][U][4];
-  W4Scales<Weights::NS> sc[2];
-  auto load = [&](int p, int step) {
-    const int unit = step * pl.kw + kw;
+  // A wave carries 64 pieces of rows wave, wave + 16, ..; rows that are not there are zeros.
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (size_t)m0 * a.K), (short)0, rows * a.K * 2, 0x00020000);
+  uint16_t* const put = xs + wave * W4_STRETCH_ROW + (lane >> 4) * 128 + 8 * w4_slot<G>(lane & 15);
+  auto fetch = [&](uint4 (&v)[MT], int step) {
+    const int k = 128 * W4_STRETCH_KW * step + 8 * lane, at = k < a.K ? 2 * (wave * a.K + k) : W4_FAR;
 #pragma unroll
-    for (int u = 0; u < U; ++u) wt.codes(w[p][u], unit * U + u);
-    wt.scales(sc[p], unit);
+    for (int t = 0; t < MT; ++t) {
+      const auto x = __builtin_amdgcn_raw_buffer_load_b128(xr, at + 32 * t * a.K, 0, 0);
+      v[t] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
   };
-  load(0, 0);
-  if (pl.units > 1) load(1, 1);
-  rx.all(xs, 0);
-  nb_f32x4 acc[MT];
-  int xrow[MT];                          // (rows past the last read it again; their results are not stored)
+  auto store = [&](const uint4 (&v)[MT], int half) {
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    acc[t] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
-    xrow[t] = min(16 * t + col, rows - 1) * rx.stride + 8 * j;
+    for (int t = 0; t < MT; ++t) *(uint4*)(put + half * HALF + 16 * t * W4_STRETCH_ROW) = nb_order8(v[t]);
+  };
+  const int steps = (a.K + 128 * W4_STRETCH_KW - 1) / (128 * W4_STRETCH_KW);
+  uint32_t w[2][4];                      // this stretch's and the next's weights
+  W4Scales<Weights::NS> sc[2];
+  uint4 v[2][MT];                        // rows of the next stretch and the one after it
+  fetch(v[0], 0);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {          // (behind the last block: zeros)
+    wt.codes(w[p], W4_STRETCH_KW * p + kw);
+    wt.scales(sc[p], W4_STRETCH_KW * p + kw);
   }
+  fetch(v[1], 1);
+  store(v[0], 0);
+  nb_f32x4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = nb_f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint16_t* const get = xs + col * W4_STRETCH_ROW + 8 * j + 128 * kw;
   auto stretch = [&](auto p_tag, int step) {
     constexpr int P = decltype(p_tag)::value;
-    const bool more = step + 1 < pl.units;
     __syncthreads();
-    // (opaque ids: the compiler would keep every piece's address in a register across the loop)
-    uint4 v[W4_PIECES];
-    if (more) {
-#pragma unroll
-      for (int i = 0; i < W4_PIECES; ++i) {
-        int id = tid + i * W4_THREADS;
-        asm volatile("" : "+v"(id));
-        if (id < total) v[i] = rx.fetch(id, (step + 1) * sblocks);
-      }
+    if (step + 2 < steps) fetch(v[P], step + 2);
+    w4_block<F16, G, MT, false, MT < 4>(acc, w[P], sc[P], 0, s16, [&](int t, int s) {
+      return *(const uint4*)(get + P * HALF + 16 * t * W4_STRETCH_ROW + 32 * s);
+    });
+    if (step + 2 < steps) {
+      wt.codes(w[P], W4_STRETCH_KW * (step + 2) + kw);
+      wt.scales(sc[P], W4_STRETCH_KW * (step + 2) + kw);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      uint32_t d[4] = {w[P][u][0], w[P][u][1], w[P][u][2], w[P][u][3]};
-      const uint16_t* at = xs + P * half + (kw * U + u) * 128;
-      w4_block<F16, G, MT, false>(acc, d, sc[P], u * (128 / G), s16, [&](int t, int s) { return *(const uint4*)(at + xrow[t] + 32 * s); });
-    }
-    if (step + 2 < pl.units) load(P, step + 2);
-    if (more) {                          // (the readers of that half passed the barrier above)
-#pragma unroll
-      for (int i = 0; i < W4_PIECES; ++i) {
-        int id = tid + i * W4_THREADS;
-        asm volatile("" : "+v"(id));
-        if (id < total) rx.put(xs + (1 - P) * half, id, v[i]);
-      }
-    }
+    if (step + 1 < steps) store(v[1 - P], 1 - P);             // (its readers passed the barrier above)
   };
-  for (int step = 0; step < pl.units; step += 2) {
+  for (int step = 0; step < steps; step += 2) {
     stretch(std::integral_constant<int, 0>(), step);
-    if (step + 1 < pl.units) stretch(std::integral_constant<int, 1>(), step + 1);
+    if (step + 1 < steps) stretch(std::integral_constant<int, 1>(), step + 1);
   }
-  if (pl.kw > 1) __syncthreads();
-  w4_finish<MT, false>(a, acc, m0, rows, wave, pl.kw, (float*)lds);
+  __syncthreads();
+  w4_finish<MT, false>(a, acc, m0, rows, wave, W4_STRETCH_KW, (float*)lds);
 }
 
+// Which kernel, measured in us with weights from memory, groups of 64, bf16 (outputs x inputs):
+//  - DIRECT while its workgroups of 16 outputs by 16 rows are few.  They read x for themselves, rows of 16
+//    the weights again:
+//      rows  outputs x inputs     DIRECT  other  |  outputs x inputs     DIRECT  other
+//        1    4096 x 4096           5.2    5.3   |   6144 x 4096           9.5    7.3
+//       16    8192 x 1024, 4096  5.3 14.2  6.2 17.0  |  12288 x 1024, 4096  7.3 19.7  6.3 17.5
+//       33    4096 x 4096          17.1   19.1   |   8192 x 4096          30.4   20.8
+//       64    1024 x 8192          13.3   39.3   |   4096 x 8192          45.1   43.2
+//  - WHOLE if two workgroups with all rows of x fit a compute unit: 60000 x 1024, groups of 32: 4 rows 12.2
+//    (STRETCH 13.5), 16 rows 14.1 (14.4), 32 rows 18.6 (23.3); 20000 x 2048: 4 rows 12.1 (14.2), 16 rows
+//    15.5 (14.9).
+//  - Waves that split the inputs leave fewer outputs to share x: as many as fill the chip one and a half
+//    times (one row, 40000 x 2048: 15.2, once 16.3; 16 rows, 30000 x 2048: 16.4, twice 21.2).
 W4Plan w4_plan(const MqW4Args& a) {
   W4Plan p;
   const int tiles = (a.N + 15) / 16, blocks = (a.K + 127) / 128, rows = a.M < 64 ? a.M : 64;
   p.mt = (rows + 15) / 16;
-  p.waves = a.M == 1 ? 4 : W4_WAVES;
-  // All of K in LDS if two workgroups of it fit a compute unit
-  p.kind = a.M <= 16 && tiles <= 512 ? W4Plan::DIRECT
+  p.waves = p.kw = a.M == 1 ? 4 : W4_WAVES;
+  p.kind = (long long)tiles * ((a.M + 15) / 16) <= (a.M == 1 ? 256 : a.M <= 16 ? 512 : 768) ? W4Plan::DIRECT
            : p.mt <= 2 && (long long)rows * a.K * 2 <= 65536 ? W4Plan::WHOLE : W4Plan::STRETCH;
-  if (p.kind == W4Plan::STRETCH) p.waves = W4_WAVES;
-  const int unit = p.kind == W4Plan::DIRECT ? 1 : p.kind == W4Plan::WHOLE ? W4_WHOLE_UNIT : W4_STRETCH_UNIT;
+  const int unit = p.kind == W4Plan::WHOLE ? W4_WHOLE_UNIT : 1;
   const int ns = unit * 128 / a.G;       // groups loaded at a time
   p.wide_scales = a.K % (ns * a.G) == 0 && ((uintptr_t)a.scales & 15) == 0 && ((uintptr_t)a.zeros & 15) == 0;
-  // Waves that split the inputs leave fewer outputs to share x: as many as fill the chip (16 waves per
-  // compute unit, 8 of the kernels with more registers)
-  const long long most = p.mt <= 2 ? 4096 : 2048;
-  p.kw = p.waves;
-  while (p.kw > 1 && (tiles * p.kw > most || unit * (p.kw / 2) >= blocks ||
-                      (p.kind == W4Plan::STRETCH && rows * 16 * unit * p.kw > W4_PIECES * W4_THREADS)))
-    p.kw /= 2;
+  if (p.kind == W4Plan::DIRECT) return p;
+  if (p.kind == W4Plan::STRETCH) {
+    p.waves = W4_STRETCH_WAVES;
+    p.kw = W4_STRETCH_KW;
+    p.lds = 2 * 16 * p.mt * W4_STRETCH_ROW * 2;        // (more than the 16 x 64 x 4 mt sums of the join)
+    return p;
+  }
+  while (p.kw > 1 && (tiles * p.kw > 6144 || unit * (p.kw / 2) >= blocks)) p.kw /= 2;
   p.units = (blocks + unit * p.kw - 1) / (unit * p.kw);
-  const int held = p.kind == W4Plan::WHOLE ? p.units * unit * p.kw : unit * p.kw, red = p.kw > 1 ? p.waves * p.mt * 1024 : 0;
-  const int x = (p.kind == W4Plan::WHOLE ? 1 : 2) * rows * (held * 256 + 16);
+  const int x = rows * (p.units * unit * p.kw * 256 + 16), red = p.kw > 1 ? p.waves * p.mt * 1024 : 0;
   p.lds = x > red ? x : red;
   return p;
 }
@@ -480,7 +489,7 @@ int mq_launch_w4_linear(const MqW4Args& a, hipStream_t stream) {
     constexpr bool F = decltype(f16)::value;
     constexpr int G = decltype(g)::value;
     if (p.kind == W4Plan::DIRECT) {
-      const dim3 grid((a.N + 15) / 16);
+      const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16);
       if (a.M == 1) hipLaunchKernelGGL((w4_direct_kernel<F, G, true>), grid, dim3(W4_THREADS), 0, stream, a, p.wide_scales);
       else hipLaunchKernelGGL((w4_direct_kernel<F, G, false>), grid, dim3(W4_THREADS), 0, stream, a, p.wide_scales);
       return;
@@ -493,9 +502,13 @@ int mq_launch_w4_linear(const MqW4Args& a, hipStream_t stream) {
       if (a.residual != nullptr) b.residual = (const char*)a.residual + (size_t)m0 * a.N * out;
       b.M = a.M - m0 < 65535 * 64 ? a.M - m0 : 65535 * 64;
       const dim3 grid(gx, (unsigned)((b.M + 16 * p.mt - 1) / (16 * p.mt)));
-      auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * p.waves), p.lds, stream, b, p); };
-      if (p.kind == W4Plan::WHOLE) launch(a.M == 1 ? w4_whole_kernel<F, G, 1, true> : p.mt == 1 ? w4_whole_kernel<F, G, 1, false> : w4_whole_kernel<F, G, 2, false>);
-      else launch(p.mt == 1 ? w4_stretch_kernel<F, G, 1> : p.mt == 2 ? w4_stretch_kernel<F, G, 2> : p.mt == 3 ? w4_stretch_kernel<F, G, 3> : w4_stretch_kernel<F, G, 4>);
+      if (p.kind == W4Plan::WHOLE) {
+        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * p.waves), p.lds, stream, b, p); };
+        launch(a.M == 1 ? w4_whole_kernel<F, G, 1, true> : p.mt == 1 ? w4_whole_kernel<F, G, 1, false> : w4_whole_kernel<F, G, 2, false>);
+      } else {
+        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * p.waves), p.lds, stream, b, p.wide_scales); };
+        launch(p.mt == 1 ? w4_stretch_kernel<F, G, 1> : p.mt == 2 ? w4_stretch_kernel<F, G, 2> : p.mt == 3 ? w4_stretch_kernel<F, G, 3> : w4_stretch_kernel<F, G, 4>);
+      }
     }
   };
   auto pick = [&](auto f16) {

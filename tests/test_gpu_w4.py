@@ -183,3 +183,18 @@ def test_argument_contracts():
         _linear(x.clone().requires_grad_(), q, s, z)
     with torch.no_grad():
         assert not _linear(x.clone().requires_grad_(), q, s, z).requires_grad
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4500, 512), (9, 8300, 512), (20, 6200, 1024), (20, 6200, 1792), (40, 4200, 896),
+                                   (64, 3100, 1536), (5, 8300, 6656), (100, 1800, 640), (65, 2600, 512), (33, 4200, 256),
+                                   (200, 900, 1024)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_outputs(m, n, k, group, dtype):
+    """Outputs enough for every way the work is laid out, inputs that end inside a block of 128 (one
+    group more than k), and row counts over several blocks of 64."""
+    k += group
+    zeros = (n // 100) % 2 == 0
+    q, s, z = _weight(n, k, group, dtype, zeros, seed=m + n + k)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(7)).to(dtype)
+    _check(_linear(x.cuda(), q.cuda(), s.cuda(), _cuda(z)), x, q, s, z, None, group)
