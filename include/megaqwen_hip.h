@@ -301,7 +301,7 @@ int mq_w4_linear(const void* d_x, const void* d_qweight, const void* d_scales, c
 /* A key/value cache in 4 bits, caller-owned: codes as bytes [batch, kv_heads, max_seq, head_dim / 2]
  * for keys and for values (zero is 8), and bf16 scales [batch, kv_heads, max_seq, 2,
  * head_dim / group_size] (a position's key scales, then its value scales).  head_dim is 64 or 128,
- * group_size 32, 64 or 128 (at most head_dim); codes 16-byte and scales 4-byte aligned.
+ * group_size 32, 64 or 128 (at most head_dim), kv_heads at most 256; codes 16-byte and scales 4-byte aligned.
  * Every call works on the last `t` positions of every sequence: lengths (device memory, int32
  * [batch]) counts a sequence's positions with these, so that row i of t is at position
  * lengths[b] - t + i.  A position outside [0, max_seq) is left out, so a batch of unequal lengths
@@ -330,7 +330,7 @@ int mq_kv4_read(const mq_kv4_cache* cache, const int32_t* d_lengths, int t, void
                 void* d_v_out, int out_dtype, void* stream);
 /* Attention over the cache: query row i of sequence b looks at positions 0 .. lengths[b] - t + i,
  *   out[b][i][h] = sum_p softmax_p(scale * q[b][i][h] . k[b][hk][p]) v[b][hk][p],
- * hk = h / (q_heads / kv_heads), at most 256 kv heads with 256 query heads each; a row that has no position to look at gives 0.  max_len bounds the
+ * hk = h / (q_heads / kv_heads), at most 256 query heads per kv head; a row that has no position to look at gives 0.  max_len bounds the
  * positions that are looked at (lengths above it are cut to it) and decides how the work is split;
  * max_seq is always right.  d_q: [batch, t, q_heads, head_dim] of dtype with element strides
  * q_strides as above; out: contiguous, of the same type.  fp32 scores, softmax and sums.

@@ -719,6 +719,7 @@ static int check_kv4(const mq_kv4_cache* c, const int32_t* d_lengths, int t, MqK
   if (c->batch < 0 || c->kv_heads < 1 || c->max_seq < 1 || t < 0)
     return fail(MQ_ERR_INVALID_ARG, "bad size (batch %d, kv_heads %d, max_seq %d, t %d)", c->batch,
                 c->kv_heads, c->max_seq, t);
+  if (c->kv_heads > 256) return fail(MQ_ERR_INVALID_ARG, "kv_heads %d exceeds 256", c->kv_heads);
   if (c->max_seq > (1 << 24)) return fail(MQ_ERR_INVALID_ARG, "max_seq %d exceeds 2^24", c->max_seq);
   if (c->head_dim != 64 && c->head_dim != 128)
     return fail(MQ_ERR_INVALID_ARG, "head_dim %d is not 64 or 128", c->head_dim);
@@ -783,8 +784,8 @@ int mq_kv4_read(const mq_kv4_cache* cache, const int32_t* d_lengths, int t, void
 static int check_attend(const mq_kv4_cache* c, int t, int q_heads, int max_len) {
   if (q_heads < 1 || q_heads % c->kv_heads != 0)
     return fail(MQ_ERR_INVALID_ARG, "q_heads %d is not a multiple of kv_heads %d", q_heads, c->kv_heads);
-  if (c->kv_heads > 256 || q_heads / c->kv_heads > 256)
-    return fail(MQ_ERR_INVALID_ARG, "more than 256 kv heads, or query heads per kv head (%d, %d)", c->kv_heads, q_heads);
+  if (q_heads / c->kv_heads > 256)
+    return fail(MQ_ERR_INVALID_ARG, "more than 256 query heads per kv head (%d of %d)", q_heads, c->kv_heads);
   if (max_len < 1 || max_len > c->max_seq)
     return fail(MQ_ERR_INVALID_ARG, "max_len %d outside [1, max_seq=%d]", max_len, c->max_seq);
   if ((long long)t * q_heads > (1 << 24) || (long long)c->batch * t * q_heads > (1ll << 24))
@@ -793,7 +794,7 @@ static int check_attend(const mq_kv4_cache* c, int t, int q_heads, int max_len) 
 }
 
 size_t mq_kv4_attend_workspace_bytes(const mq_kv4_cache* cache, int t, int q_heads, int max_len) {
-  if (cache == nullptr || cache->kv_heads < 1 || cache->batch < 1 || t < 1 ||
+  if (cache == nullptr || cache->kv_heads < 1 || cache->kv_heads > 256 || cache->batch < 1 || t < 1 ||
       check_attend(cache, t, q_heads, max_len) != MQ_OK)
     return 0;
   return mq_kv4_attend_workspace(cache->batch, t, q_heads, cache->kv_heads, cache->head_dim,

@@ -15,22 +15,41 @@ MQ_DEV uint16_t to16(float v, bool f16) {
   return f16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : f32_to_bf16(v);
 }
 
-// One thread per 8 values of a key (which = 0) or value row, neighbours along the row:
+// Rows of 8-value pieces: a thread takes one of (t, piece), the grid's second dimension is (key or
+// value, kv head) and its third the sequence.  A head's rows are neighbours in the cache, so that a
+// wave writes (append) or reads 256 bytes of codes in a row; on the other side every row of a head
+// is D 2 bytes in a row.
+struct KvPiece {
+  int t, piece, h;
+  bool which, in;                  // value rows; a row of the call
+  long long pos;                   // the cache row, or < 0 or >= S
+};
+MQ_DEV KvPiece kv_piece(const MqKv4& c, int b) {
+  const int shift = c.D == 128 ? 4 : 3, id = blockIdx.x * 256 + threadIdx.x;
+  KvPiece p;
+  p.t = id >> shift;
+  p.piece = id & ((1 << shift) - 1);
+  p.which = blockIdx.y >= (unsigned)c.Hkv;
+  p.h = p.which ? blockIdx.y - c.Hkv : blockIdx.y;
+  p.in = p.t < c.T;
+  p.pos = (long long)c.lengths[b] - c.T + p.t;
+  return p;
+}
+
 //   s = bf16(max|x| / 7) over the group's G / 8 threads, u = clamp(rint(x / s), -7, 7) + 8; s = 0:
 //   u = 8; a group that holds an infinity or a NaN gets s = NaN, so that all of its values read as NaN.
-// The quotient is the correctly rounded fp32 one: a bf16 or fp16 value over a bf16 scale is never so
-// close to half a step that this could round to the other side of it.
+// Quotients are reciprocals with one correction, q' = q + (x - q s) r: off by an ulp or two of fp32 at
+// most, and exact where x / s has few bits.  x has up to 11 bits and s 8, so x / s is either exactly
+// half a step, and then so is q', or at least 2^-12 of it away: no code differs from the exact
+// quotient's.  The same holds for max / 7 and the midpoints of bf16.  Below 2^-60 the products could
+// underflow, and the quotients are divisions.
 template <bool F16, int G>
 __global__ void __launch_bounds__(256) kv4_append_kernel(MqKv4 c, const uint16_t* k, MqStrides ks, const uint16_t* v, MqStrides vs) {
-  const unsigned per = c.D / 8, n = (unsigned)c.T * c.Hkv * per, id = blockIdx.x * 256 + threadIdx.x;
-  const int b = blockIdx.y;
-  if (id >= 2 * n) return;
-  const bool which = id >= n;
-  const unsigned at = which ? id - n : id, piece = at % per, row_id = at / per;
-  const int h = row_id % c.Hkv, t = row_id / c.Hkv;
-  const MqStrides st = which ? vs : ks;
-  const uint4 x = nb_load16((which ? v : k) + b * st.b + t * st.t + h * st.h + 8 * piece);
-  const long long pos = (long long)c.lengths[b] - c.T + t;
+  const int b = blockIdx.z;
+  const KvPiece p = kv_piece(c, b);
+  if (!p.in) return;               // (whole groups)
+  const MqStrides st = p.which ? vs : ks;
+  const uint4 x = nb_load16((p.which ? v : k) + b * st.b + p.t * st.t + p.h * st.h + 8 * p.piece);
   const float f[8] = {nb_lo<F16>(x.x), nb_hi<F16>(x.x), nb_lo<F16>(x.y), nb_hi<F16>(x.y),
                       nb_lo<F16>(x.z), nb_hi<F16>(x.z), nb_lo<F16>(x.w), nb_hi<F16>(x.w)};
   // (maximum keeps a NaN; the lanes of a group are in the same row of 16)
@@ -41,41 +60,52 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(MqKv4 c, const uint16_t
   m = __builtin_elementwise_maximum(m, dpp_f<MQ_DPP_QUAD_XOR2>(m));
   if constexpr (G >= 64) m = __builtin_elementwise_maximum(m, dpp_f<MQ_DPP_ROW_HALF_MIRROR>(m));
   if constexpr (G >= 128) m = __builtin_elementwise_maximum(m, dpp_f<MQ_DPP_ROW_MIRROR>(m));
-  const uint16_t sb = m < INFINITY ? f32_to_bf16(m / 7.0f) : 0x7fc0;
-  const float s = bf16_to_f32(sb);
+  auto quotient = [](float a, float d, float r) {
+    const float q = a * r;
+    return fmaf(fmaf(-q, d, a), r, q);
+  };
   uint32_t w = 0;
+  uint16_t sb;
+  if (m >= 0x1p-60f && m < INFINITY) {
+    sb = f32_to_bf16(quotient(m, 7.0f, 1.0f / 7.0f));
+    const float s = bf16_to_f32(sb), r = __builtin_amdgcn_rcpf(s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float r = s > 0.f ? rintf(f[i] / s) : 0.f;
-    w |= (uint32_t)(int)(fminf(fmaxf(r, -7.f), 7.f) + 8.f) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      // the sum's last bits: its rounding is rint's, 8 is added, and the constant ends in four zeros
+      const float u = __builtin_amdgcn_fmed3f(quotient(f[i], s, r), -7.f, 7.f) + (0x1.8p23f + 8.f);
+      w |= (__float_as_uint(u) & 15u) << (4 * i);
+    }
+  } else {
+    sb = m < INFINITY ? f32_to_bf16(m / 7.0f) : 0x7fc0;
+    const float s = bf16_to_f32(sb);
+    for (int i = 0; i < 8; ++i) {
+      const float r = s > 0.f ? rintf(f[i] / s) : 0.f;
+      w |= (uint32_t)(int)(fminf(fmaxf(r, -7.f), 7.f) + 8.f) << (4 * i);
+    }
   }
-  if (pos < 0 || pos >= c.S) return;
-  const size_t row = ((size_t)b * c.Hkv + h) * c.S + pos;
-  ((uint32_t*)(which ? c.vq : c.kq))[row * per + piece] = w;
-  if (piece % (G / 8) == 0) c.scales[(row * 2 + which) * (c.D / G) + piece / (G / 8)] = sb;
+  if (p.pos < 0 || p.pos >= c.S) return;
+  const size_t row = ((size_t)b * c.Hkv + p.h) * c.S + p.pos;
+  ((uint32_t*)(p.which ? c.vq : c.kq))[row * (c.D / 8) + p.piece] = w;
+  if (p.piece % (G / 8) == 0) c.scales[(row * 2 + p.which) * (c.D / G) + p.piece / (G / 8)] = sb;
 }
 
-// One thread per 8 values; rows outside [0, S) read as 0.
+// Rows outside [0, S) read as 0.
 __global__ void __launch_bounds__(256) kv4_read_kernel(MqKv4 c, void* k, void* v, int o_type) {
-  const unsigned per = c.D / 8, n = (unsigned)c.T * c.Hkv * per, id = blockIdx.x * 256 + threadIdx.x;
-  const int b = blockIdx.y;
-  if (id >= 2 * n) return;
-  const bool which = id >= n;
-  const unsigned at = which ? id - n : id, piece = at % per, row_id = at / per;
-  const int h = row_id % c.Hkv, t = row_id / c.Hkv;
-  const long long pos = (long long)c.lengths[b] - c.T + t;
+  const int b = blockIdx.z, per = c.D / 8, gshift = c.G == 32 ? 2 : c.G == 64 ? 3 : 4;
+  const KvPiece p = kv_piece(c, b);
+  if (!p.in) return;
   float s = 0.f;
   uint32_t u = 0;
-  if (pos >= 0 && pos < c.S) {
-    const size_t row = ((size_t)b * c.Hkv + h) * c.S + pos;
-    s = bf16_to_f32(c.scales[(row * 2 + which) * (c.D / c.G) + 8 * piece / c.G]);
-    u = ((const uint32_t*)(which ? c.vq : c.kq))[row * per + piece];
+  if (p.pos >= 0 && p.pos < c.S) {
+    const size_t row = ((size_t)b * c.Hkv + p.h) * c.S + p.pos;
+    s = bf16_to_f32(c.scales[(row * 2 + p.which) * (per >> gshift) + (p.piece >> gshift)]);
+    u = ((const uint32_t*)(p.which ? c.vq : c.kq))[row * per + p.piece];
   }
   float f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = s * (float)((int)((u >> (4 * i)) & 15u) - 8);
-  const size_t o = ((size_t)b * n + at) * 8;
-  void* out = which ? v : k;
+  const size_t o = ((((size_t)b * c.T + p.t) * c.Hkv + p.h) * per + p.piece) * 8;
+  void* out = p.which ? v : k;
   if (o_type == MQ_T_F32) {
     float4* dst = (float4*)((float*)out + o);
     dst[0] = make_float4(f[0], f[1], f[2], f[3]);
@@ -542,11 +572,8 @@ int launched() { return hipGetLastError() == hipSuccess ? 0 : -1; }
 
 }  // namespace
 
-// (8 values per thread; the host has checked T Hkv <= 2^26)
-static dim3 kv4_row_grid(const MqKv4& c) {
-  const unsigned n = 2u * (unsigned)c.T * c.Hkv * (c.D / 8);
-  return dim3((n + 255) / 256, c.B);
-}
+// (the host has checked T Hkv <= 2^26 and Hkv <= 256)
+static dim3 kv4_row_grid(const MqKv4& c) { return dim3(((unsigned)c.T * (c.D / 8) + 255) / 256, 2 * c.Hkv, c.B); }
 
 int mq_launch_kv4_append(const MqKv4& c, const uint16_t* k, MqStrides ks, const uint16_t* v,
                          MqStrides vs, bool f16, hipStream_t stream) {

@@ -44,8 +44,9 @@ class KV4Cache:
                  max_seq_len: int = 2048, head_dim: int = COMPILED_LAYER_SHAPE["head_dim"],
                  group_size: int = 32, *, device="cuda"):
         shape = (int(batch), int(num_kv_heads), int(max_seq_len))
-        if min(shape) < 1:
-            raise ValueError(f"batch, num_kv_heads and max_seq_len must be positive, got {shape}")
+        if min(shape) < 1 or shape[1] > 256:
+            raise ValueError("batch, num_kv_heads and max_seq_len must be positive, and num_kv_heads at most 256, "
+                             f"got {shape}")
         if head_dim not in HEAD_DIMS or group_size not in GROUP_SIZES or group_size > head_dim:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS} and group_size one of {GROUP_SIZES}, "
                              f"at most head_dim; got {head_dim} and {group_size}")
@@ -61,9 +62,9 @@ class KV4Cache:
         """A cache over caller-owned tensors of the shapes above (they are used in place)."""
         if k_codes.ndim != 4 or k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 \
                 or v_codes.shape != k_codes.shape or k_codes.shape[-1] * 2 not in HEAD_DIMS \
-                or min(k_codes.shape) < 1:
+                or min(k_codes.shape) < 1 or k_codes.shape[1] > 256:
             raise ValueError("k_codes and v_codes must be uint8 [batch, kv_heads, max_seq_len, head_dim / 2] with "
-                             f"head_dim one of {HEAD_DIMS}; got {k_codes.dtype} {tuple(k_codes.shape)} and "
+                             f"head_dim one of {HEAD_DIMS} and at most 256 kv_heads; got {k_codes.dtype} {tuple(k_codes.shape)} and "
                              f"{v_codes.dtype} {tuple(v_codes.shape)}")
         dim = 2 * k_codes.shape[-1]
         if scales.ndim != 5 or scales.dtype != torch.bfloat16 or scales.shape[:4] != (*k_codes.shape[:3], 2) \
@@ -146,8 +147,8 @@ class KV4Cache:
     def attend(self, q: torch.Tensor, lengths: torch.Tensor, *, scale: Optional[float] = None,
                max_length: Optional[int] = None) -> torch.Tensor:
         """Causal attention of q [batch, t, q_heads, head_dim] (bf16 or fp16, q_heads a multiple of
-        kv_heads, neither kv heads nor query heads per kv head above 256) over the cache: query i of t looks at positions 0 .. lengths[b] - t + i.  The
-        output has q's type and shape; a query with no position to look at gives 0.  `scale`
+        kv_heads, by at most 256) over the cache: query i of t looks at positions
+        0 .. lengths[b] - t + i.  The output has q's type and shape; a query with no position to look at gives 0.  `scale`
         defaults to 1/sqrt(head_dim).  max_length, if known, is an upper bound of `lengths`: the
         work is split for it, and positions from there on are not looked at."""
         q = self._rows("KV4Cache.attend", "q", q, None)

@@ -332,3 +332,29 @@ def test_attend_odd_and_largest_head_counts(b, t, h, r, s):
     _fill(c, seed=31)
     q, lens = _randn((b, t, h * r, 128), 32), [s - 5 * i for i in range(b)]
     _check_attend(c, q, lens, c.attend(q, _lengths(lens)))
+
+
+@pytest.mark.parametrize("dtype,top", [(torch.bfloat16, 0), (torch.bfloat16, -62), (torch.bfloat16, -60), (torch.bfloat16, 127),
+                                       (torch.bfloat16, -126), (torch.float16, 0), (torch.float16, 15)])
+def test_append_every_pair_of_mantissas(dtype, top):
+    """Codes and scales are those of exact quotients: every mantissa as a group's maximum 2^top .. with
+    every mantissa of the four binades up to it (every 7th for fp16), ties among them."""
+    bits = 7 if dtype == torch.bfloat16 else 10
+    mant = 1 + torch.arange(1 << bits, dtype=torch.float64) / (1 << bits)
+    x = torch.cat([mant * 2.0 ** -e for e in range(4)])[::1 if bits == 7 else 7]
+    x = torch.cat([x, torch.zeros(-x.numel() % 31, dtype=x.dtype)])
+    rows = []
+    for m in mant:
+        y = torch.where(x <= m, x, x / 2).view(-1, 31)
+        rows.append(torch.cat([m.expand(y.shape[0], 1), y * torch.where(torch.arange(31) % 2 == 0, 1.0, -1.0)], 1))
+    y = (torch.cat(rows) * 2.0 ** top).to(dtype)                 # exact, but for bf16's smallest
+    y = torch.cat([y, torch.zeros(-y.shape[0] % 4, 32, dtype=dtype)]).view(1, -1, 1, 128)
+    t = y.shape[1]
+    c = _cache(1, 1, t, 128, 32)
+    c.append(y.cuda(), -y.cuda(), _lengths([t]))
+    u, s = q4_ref.kv4_quantize(_np(y)[0, :, 0], 32)
+    assert np.array_equal(c.scales[0, 0, :, 0].double().cpu().numpy(), s)
+    assert np.array_equal(c.scales[0, 0, :, 1].double().cpu().numpy(), s)
+    for codes, want in ((c.k_codes, u), (c.v_codes, 16 - u)):
+        got = torch.stack([codes[0, 0] & 15, codes[0, 0] >> 4], -1).flatten(-2).cpu().numpy()
+        assert np.array_equal(got, want)

@@ -97,3 +97,17 @@ def test_c_abi_attend_head_limits():
                                  None) == _lib.MQ_ERR_INVALID_ARG
         assert b"256" in lib.mq_last_error()
         assert lib.mq_kv4_attend_workspace_bytes(c, 1, hq, 100) == 0
+
+
+def test_at_most_256_kv_heads():
+    with pytest.raises(ValueError, match="256"):
+        KV4Cache(1, 257, 8)
+    c, s = torch.zeros(1, 257, 1, 64, dtype=torch.uint8), torch.zeros(1, 257, 1, 2, 4, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="256"):
+        KV4Cache.from_tensors(c, c, s)
+    lib, A = _lib.load(), 1 << 24
+    st = (ctypes.c_int64 * 3)(1 << 20, 1 << 20, 128)
+    c = ctypes.byref(_lib.Kv4Cache(A, 2 * A, 3 * A, 1, 257, 100, 128, 32))
+    assert lib.mq_kv4_append(c, 4 * A, st, 5 * A, st, 6 * A, 1, _lib.MQ_DTYPE_BF16, None) == _lib.MQ_ERR_INVALID_ARG
+    assert b"256" in lib.mq_last_error()
+    assert lib.mq_kv4_read(c, 6 * A, 1, 4 * A, 5 * A, _lib.MQ_DTYPE_BF16, None) == _lib.MQ_ERR_INVALID_ARG
