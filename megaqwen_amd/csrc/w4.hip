@@ -80,9 +80,22 @@ template <int G> MQ_DEV int w4_slot(int piece) {
   else return 4 * p + d;
 }
 
+// Rows n0 .. n0 + rows of a tensor (in scalar registers)
+MQ_DEV int w4_outputs(const MqW4Args& a, int n0) { return __builtin_amdgcn_readfirstlane(max(0, min(16, a.N - n0))); }
+MQ_DEV __amdgpu_buffer_rsrc_t w4_rsrc(const void* p, int row_bytes, int n0, int rows) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)p + (size_t)n0 * row_bytes), (short)0, rows * row_bytes, 0x00020000);
+}
+MQ_DEV void w4_codes(uint32_t (&w)[4], __amdgpu_buffer_rsrc_t wr, int K, int col, int j, int b) {
+  const int k = 128 * b + 32 * j;
+  const auto v = __builtin_amdgcn_raw_buffer_load_b128(wr, k < K ? col * (K / 2) + k / 2 : W4_FAR, 0, 0);
+  for (int i = 0; i < 4; ++i) w[i] = v[i];
+}
+
 // Scales and zero points of the NS groups of U blocks of 128 inputs of one output.
 template <int NS> struct W4Scales {
   uint32_t s[(NS + 1) / 2], z[(NS + 3) / 4];
+  MQ_DEV uint32_t scale(int g) const { return g & 1 ? s[g / 2] >> 16 : s[g / 2]; }     // in the low 16 bits
+  MQ_DEV uint32_t zero(int g) const { return (z[g / 4] >> (8 * (g & 3))) & 255u; }
 };
 // Loads the weights of the 16 outputs from n0 on, U blocks at a time: those of outputs >= N and inputs >= K
 // return 0 without an access.
@@ -98,23 +111,17 @@ template <int G, int U> struct W4Weights {
     j = lane >> 4;
     wide = wide_scales;
     zeros = a.zeros != nullptr;
-    const int rows = __builtin_amdgcn_readfirstlane(max(0, min(16, a.N - n0)));   // (resources stay in scalar registers)
-    wr = rsrc(a.qw, K / 2, n0, rows);
-    sr = rsrc(a.scales, groups * 2, n0, rows);
-    zr = rsrc(a.zeros, groups, n0, rows);
-  }
-  static MQ_DEV __amdgpu_buffer_rsrc_t rsrc(const void* p, int row_bytes, int n0, int rows) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)p + (size_t)n0 * row_bytes), (short)0, rows * row_bytes, 0x00020000);
+    const int rows = w4_outputs(a, n0);
+    wr = w4_rsrc(a.qw, K / 2, n0, rows);
+    sr = w4_rsrc(a.scales, groups * 2, n0, rows);
+    zr = w4_rsrc(a.zeros, groups, n0, rows);
   }
   // words of block b
-  MQ_DEV void codes(uint32_t (&w)[4], int b) const {
-    const int k = 128 * b + 32 * j;
-    const auto v = __builtin_amdgcn_raw_buffer_load_b128(wr, k < K ? col * (K / 2) + k / 2 : W4_FAR, 0, 0);
-    for (int i = 0; i < 4; ++i) w[i] = v[i];
-  }
-  // groups of blocks U unit .. U unit + U
+  MQ_DEV void codes(uint32_t (&w)[4], int b) const { w4_codes(w, wr, K, col, j, b); }
+  // groups of blocks U unit .. U unit + U; those >= groups have scale 0 (and not the next output's first,
+  // which may be infinite)
   MQ_DEV void scales(W4Scales<NS>& x, int unit) const {
-    int g = col * groups + NS * unit;
+    int g = NS * unit < groups ? col * groups + NS * unit : W4_FAR / 2;
     asm volatile("" : "+v"(g));          // (opaque: or every group's offset below has a register of its own)
     for (int i = 0; i < (NS + 3) / 4; ++i) x.z[i] = 0x08080808u;
     if (wide) {                          // NS groups are there, and aligned
@@ -155,10 +162,10 @@ template <int G, int U> struct W4Weights {
 };
 
 // acc[t] += the products of a block whose first group is the first-th of sc (s16: all ones if the scales are
-// fp16, 0 for bf16); x_of(t, step) is the operand of row tile t.  A step's operands are read one step ahead, and no further: steps mixed by the scheduler
-// take more registers than there are.
-template <bool F16, int G, int MT, bool ONE, bool AHEAD = true, int NS, class X>
-MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& sc, int first, uint32_t s16, X x_of) {
+// fp16, 0 for bf16); x_of(t, step) is the operand of row tile t.  AHEAD: a step's operands are read one step
+// ahead, and no further: steps mixed by the scheduler take more registers than there are.
+template <bool F16, int G, int MT, bool ONE, bool AHEAD = true, class S, class X>
+MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const S& sc, int first, uint32_t s16, X x_of) {
   constexpr int SPG = G / 32;            // steps of a group
   w4_exchange<G>(d);
   uint4 x[MT], zero;
@@ -178,7 +185,7 @@ MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& 
     }
     const int g = first + s / SPG;
     if (s % SPG == 0) {
-      const uint32_t z = (sc.z[g / 4] >> (8 * (g & 3))) & 255u, zc = F16 ? 0xcc00u + (z << 6) : 0xc180u + (z << 3);
+      const uint32_t z = sc.zero(g), zc = F16 ? 0xcc00u + (z << 6) : 0xc180u + (z << 3);
       const uint32_t zz = zc | (zc << 16);                    // -(16 + z), twice
       zero = make_uint4(zz, zz, zz, zz);
 #pragma unroll
@@ -192,7 +199,7 @@ MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const W4Scales<NS>& 
     }
     if (s % SPG == SPG - 1) {
       // (both readings and a select: a branch here moves all groups' sums to the end of the block)
-      const uint32_t sw = g & 1 ? sc.s[g / 2] >> 16 : sc.s[g / 2], half = __float_as_uint(w4_from16(sw & 0xffffu, true));
+      const uint32_t sw = sc.scale(g), half = __float_as_uint(w4_from16(sw & 0xffffu, true));
       const float f = __uint_as_float((half & s16) | ((sw << 16) & ~s16));
 #pragma unroll
       for (int t = 0; t < MT; ++t)
@@ -274,6 +281,12 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (wave + W4_WAVES * u < blocks) load(y[u], wave + W4_WAVES * u);
+  // One output per thread at the end; its residual is on the way from here.
+  constexpr int R = ONE ? 1 : 4;
+  const int om = 4 * j + (wave & (R - 1)), on = 16 * blockIdx.x + col;
+  const bool mine = wave < R && om < rows && on < a.N;
+  const size_t out_at = (size_t)(m0 + om) * a.N + on;
+  const float residual = mine && a.residual != nullptr ? w4_residual(a.residual, out_at, a.o_type) : 0.f;
   for (int b = wave; b < blocks; b += W4_WAVES * U) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -282,7 +295,14 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
       if (b + W4_WAVES * (u + U) < blocks) load(y[u], b + W4_WAVES * (u + U));
     }
   }
-  w4_finish<1, ONE>(a, acc, m0, rows, wave, W4_WAVES, red);
+#pragma unroll
+  for (int i = 0; i < R; ++i) red[(wave * R + i) * 64 + lane] = acc[0][i];
+  __syncthreads();
+  if (!mine) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int q = 0; q < W4_WAVES; ++q) sum += red[(q * R + wave) * 64 + lane];
+  w4_store(a.out, out_at, sum + residual, a.o_type);
 }
 
 struct W4Plan {
@@ -379,16 +399,76 @@ __global__ void __launch_bounds__(W4_THREADS, MT == 2 ? 2 : G == 32 && !ONE ? 3 
   w4_finish<MT, ONE>(a, acc, m0, rows, wave, pl.kw, (float*)lds);
 }
 
-template <bool F16, int G, int MT>
-__global__ void __launch_bounds__(64 * W4_STRETCH_WAVES, 4) w4_stretch_kernel(MqW4Args a, bool wide_scales) {
-  typedef W4Weights<G, 1> Weights;
+// Scales and zero points of the groups of a block of 128 inputs of one output, packed (WIDE) or one to a
+// register.
+template <int G, bool WIDE> struct W4BlockScales {
+  static constexpr int NS = 128 / G;
+  uint32_t s[WIDE ? (NS + 1) / 2 : NS], z[WIDE ? 1 : NS], flip;
+  MQ_DEV uint32_t scale(int g) const { return WIDE ? (g & 1 ? s[g / 2] >> 16 : s[g / 2]) : s[g]; }     // in the low 16 bits
+  MQ_DEV uint32_t zero(int g) const { return ((WIDE ? z[0] ^ flip : z[g] ^ flip) >> (WIDE ? 8 * g : 0)) & 255u; }
+};
+// W4Weights a block at a time and without a branch: the compiler's wait for a load that may or may not have
+// been followed by others is a wait for all of them, which costs the stretches 10%.  (In the other kernels
+// the loads that a branch saves are worth more, about 20 cycles of a compute unit each: the vocabulary's
+// product of one row took 20.4 us for 16.4, the q|k|v product of one row 3.7 for 2.6.)
+// WIDE: a block's scales are one aligned load, and its zero points.
+template <int G, bool WIDE> struct W4Block {
+  typedef W4BlockScales<G, WIDE> Scales;
+  static constexpr int NS = Scales::NS;
+  __amdgpu_buffer_rsrc_t wr, sr, zr;
+  int K, groups, col, j;
+  uint32_t no_zeros;                     // no zero points: they read as 0, and these bits make them 8
+  MQ_DEV W4Block(const MqW4Args& a, int n0, int lane) {
+    K = a.K;
+    groups = K / G;
+    col = lane & 15;
+    j = lane >> 4;
+    no_zeros = a.zeros == nullptr ? 0x08080808u : 0u;
+    const int rows = w4_outputs(a, n0);
+    wr = w4_rsrc(a.qw, K / 2, n0, rows);
+    sr = w4_rsrc(a.scales, groups * 2, n0, rows);
+    zr = w4_rsrc(a.zeros, groups, n0, a.zeros == nullptr ? 0 : rows);
+  }
+  // words of block b
+  MQ_DEV void codes(uint32_t (&w)[4], int b) const { w4_codes(w, wr, K, col, j, b); }
+  // its groups; those behind the last have scale 0 (and not the next output's first, which may be infinite)
+  MQ_DEV void scales(Scales& x, int b) const {
+    x.flip = no_zeros;
+    if constexpr (WIDE) {
+      int g = NS * b < groups ? col * groups + NS * b : W4_FAR / 2;
+      if constexpr (NS == 1) {
+        x.s[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, 2 * g, 0, 0);
+        x.z[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zr, g, 0, 0);
+      } else if constexpr (NS == 2) {
+        x.s[0] = __builtin_amdgcn_raw_buffer_load_b32(sr, 2 * g, 0, 0);
+        x.z[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(zr, g, 0, 0);
+      } else {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(sr, 2 * g, 0, 0);
+        x.s[0] = v[0];
+        x.s[1] = v[1];
+        x.z[0] = __builtin_amdgcn_raw_buffer_load_b32(zr, g, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int g = NS * b + i < groups ? col * groups + NS * b + i : W4_FAR / 2;
+        x.s[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, 2 * g, 0, 0);
+        x.z[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zr, g, 0, 0);
+      }
+    }
+  }
+};
+
+template <bool F16, int G, bool WIDE, int MT>
+__global__ void __launch_bounds__(64 * W4_STRETCH_WAVES, 4) w4_stretch_kernel(MqW4Args a) {
+  typedef W4Block<G, WIDE> Weights;
   constexpr int HALF = 16 * MT * W4_STRETCH_ROW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   uint16_t* xs = (uint16_t*)lds;                       // [2] stretches of [16 MT] rows
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, j = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = wave / W4_STRETCH_KW, kw = wave % W4_STRETCH_KW;
   const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
-  const Weights wt(a, (blockIdx.x * W4_STRETCH_TILES + nw) * 16, wide_scales, lane);
+  const Weights wt(a, (blockIdx.x * W4_STRETCH_TILES + nw) * 16, lane);
   const uint32_t s16 = a.s_type == MQ_T_F16 ? ~0u : 0u;
   // A wave carries 64 pieces of rows wave, wave + 16, ..; rows that are not there are zeros.
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (size_t)m0 * a.K), (short)0, rows * a.K * 2, 0x00020000);
@@ -407,7 +487,7 @@ __global__ void __launch_bounds__(64 * W4_STRETCH_WAVES, 4) w4_stretch_kernel(Mq
   };
   const int steps = (a.K + 128 * W4_STRETCH_KW - 1) / (128 * W4_STRETCH_KW);
   uint32_t w[2][4];                      // this stretch's and the next's weights
-  W4Scales<Weights::NS> sc[2];
+  typename Weights::Scales sc[2];
   uint4 v[2][MT];                        // rows of the next stretch and the one after it
   fetch(v[0], 0);
 #pragma unroll
@@ -424,15 +504,13 @@ __global__ void __launch_bounds__(64 * W4_STRETCH_WAVES, 4) w4_stretch_kernel(Mq
   auto stretch = [&](auto p_tag, int step) {
     constexpr int P = decltype(p_tag)::value;
     __syncthreads();
-    if (step + 2 < steps) fetch(v[P], step + 2);
+    fetch(v[P], step + 2);
     w4_block<F16, G, MT, false, MT < 4>(acc, w[P], sc[P], 0, s16, [&](int t, int s) {
       return *(const uint4*)(get + P * HALF + 16 * t * W4_STRETCH_ROW + 32 * s);
     });
-    if (step + 2 < steps) {
-      wt.codes(w[P], W4_STRETCH_KW * (step + 2) + kw);
-      wt.scales(sc[P], W4_STRETCH_KW * (step + 2) + kw);
-    }
-    if (step + 1 < steps) store(v[1 - P], 1 - P);             // (its readers passed the barrier above)
+    wt.codes(w[P], W4_STRETCH_KW * (step + 2) + kw);
+    wt.scales(sc[P], W4_STRETCH_KW * (step + 2) + kw);
+    store(v[1 - P], 1 - P);              // (its readers passed the barrier above)
   };
   for (int step = 0; step < steps; step += 2) {
     stretch(std::integral_constant<int, 0>(), step);
@@ -443,13 +521,13 @@ __global__ void __launch_bounds__(64 * W4_STRETCH_WAVES, 4) w4_stretch_kernel(Mq
 }
 
 // Which kernel, measured in us with weights from memory, groups of 64, bf16 (outputs x inputs):
-//  - DIRECT while its workgroups of 16 outputs by 16 rows are few.  They read x for themselves, rows of 16
-//    the weights again:
-//      rows  outputs x inputs     DIRECT  other  |  outputs x inputs     DIRECT  other
-//        1    4096 x 4096           5.2    5.3   |   6144 x 4096           9.5    7.3
-//       16    8192 x 1024, 4096  5.3 14.2  6.2 17.0  |  12288 x 1024, 4096  7.3 19.7  6.3 17.5
-//       33    4096 x 4096          17.1   19.1   |   8192 x 4096          30.4   20.8
-//       64    1024 x 8192          13.3   39.3   |   4096 x 8192          45.1   43.2
+//  - DIRECT while its workgroups of 16 outputs by 16 rows are few.  They read x for themselves, and further
+//    tiles of rows the weights again:
+//      rows  outputs x inputs        DIRECT     other    |  outputs x inputs        DIRECT     other
+//        1    4096 x 4096               5.2       5.3    |   6144 x 4096               9.5       7.3
+//       16    8192 x 1024, 8192    5.3 25.1   6.2 23.3   |  12288 x 1024, 8192    7.3 35.6   6.3 32.1
+//       33    4096 x 1024, 8192    6.4 30.5   8.5 33.7   |   8192 x 1024, 8192   10.4 57.2   8.6 33.7
+//       64    2048 x 1024, 8192    5.1 23.6   9.6 35.0   |   4096 x 1024, 8192    8.6 45.1   9.8 38.2
 //  - WHOLE if two workgroups with all rows of x fit a compute unit: 60000 x 1024, groups of 32: 4 rows 12.2
 //    (STRETCH 13.5), 16 rows 14.1 (14.4), 32 rows 18.6 (23.3); 20000 x 2048: 4 rows 12.1 (14.2), 16 rows
 //    15.5 (14.9).
@@ -506,8 +584,14 @@ int mq_launch_w4_linear(const MqW4Args& a, hipStream_t stream) {
         auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * p.waves), p.lds, stream, b, p); };
         launch(a.M == 1 ? w4_whole_kernel<F, G, 1, true> : p.mt == 1 ? w4_whole_kernel<F, G, 1, false> : w4_whole_kernel<F, G, 2, false>);
       } else {
-        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * p.waves), p.lds, stream, b, p.wide_scales); };
-        launch(p.mt == 1 ? w4_stretch_kernel<F, G, 1> : p.mt == 2 ? w4_stretch_kernel<F, G, 2> : p.mt == 3 ? w4_stretch_kernel<F, G, 3> : w4_stretch_kernel<F, G, 4>);
+        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * p.waves), p.lds, stream, b); };
+        auto tiles = [&](auto wide) {
+          constexpr bool W = decltype(wide)::value;
+          launch(p.mt == 1 ? w4_stretch_kernel<F, G, W, 1> : p.mt == 2 ? w4_stretch_kernel<F, G, W, 2> : p.mt == 3 ? w4_stretch_kernel<F, G, W, 3> : w4_stretch_kernel<F, G, W, 4>);
+        };
+        if constexpr (G == 128) tiles(std::true_type());             // (always one load)
+        else if (p.wide_scales) tiles(std::true_type());
+        else tiles(std::false_type());
       }
     }
   };

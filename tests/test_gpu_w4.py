@@ -198,3 +198,16 @@ def test_many_outputs(m, n, k, group, dtype):
     q, s, z = _weight(n, k, group, dtype, zeros, seed=m + n + k)
     x = torch.randn(m, k, generator=torch.Generator().manual_seed(7)).to(dtype)
     _check(_linear(x.cuda(), q.cuda(), s.cuda(), _cuda(z)), x, q, s, z, None, group)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 40, 640), (1, 4500, 640), (9, 8300, 640), (20, 6200, 1920), (40, 4200, 640)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_an_infinite_scale_stays_in_its_output(m, n, k, group):
+    """Inputs that end inside the last turn of a workgroup: what is read for the rest is not the next
+    output's scale."""
+    q, s, z = _weight(n, k, group, torch.bfloat16, True, seed=11)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16)
+    want = _linear(x.cuda(), q.cuda(), s.cuda(), z.cuda()).cpu()
+    s[1::2] = float("inf")
+    got = _linear(x.cuda(), q.cuda(), s.cuda(), z.cuda()).cpu()
+    assert torch.equal(got[:, ::2], want[:, ::2]) and not torch.isfinite(got[:, 1::2]).any()
