@@ -242,10 +242,10 @@ __global__ void __launch_bounds__(64 * WAVES, CT == 1 ? 4 : 2) kv4_attend_kernel
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int pos = p + 16 * t + 4 * j + i, e = 4 * t + i;
-        if constexpr (NG == 2) {         // both groups of key and value
-          const auto w = __builtin_amdgcn_raw_buffer_load_b64(sr, pos * 8, 0, 0);
-          x.s[2 * e] = w[0];
-          x.s[2 * e + 1] = w[1];
+        if constexpr (NG == 2) {         // both groups of key and value, two positions at a time
+          if (i & 1) continue;
+          const auto w = __builtin_amdgcn_raw_buffer_load_b128(sr, pos * 8, 0, 0);
+          for (int q = 0; q < 4; ++q) x.s[2 * e + q] = w[q];
         } else if constexpr (NG == 4) {
           x.s[2 * e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * 16 + 2 * g, 0, 0);
           x.s[2 * e + 1] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, pos * 16 + 8 + 2 * g, 0, 0);
