@@ -52,12 +52,6 @@ template <bool F16> MQ_DEV float nb_lo(uint32_t w) {
 template <bool F16> MQ_DEV float nb_hi(uint32_t w) {
   return F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)) : bf16_hi(w);
 }
-// Sum of the 8 elements of an operand, in fp32
-template <bool F16> MQ_DEV float nb_sum8(uint4 x) {
-  return ((nb_lo<F16>(x.x) + nb_hi<F16>(x.x)) + (nb_lo<F16>(x.y) + nb_hi<F16>(x.y))) +
-         ((nb_lo<F16>(x.z) + nb_hi<F16>(x.z)) + (nb_lo<F16>(x.w) + nb_hi<F16>(x.w)));
-}
-
 // 16 bytes at any 2-byte aligned address
 struct __attribute__((packed, aligned(2))) NbLoose16 {
   uint32_t w[4];

@@ -19,6 +19,12 @@
 //   w4_whole_kernel    several tiles of 16 outputs per workgroup share the rows of x, which wait in LDS in
 //                      operand order; kw waves split a tile's inputs
 //   w4_stretch_kernel  the same where the rows do not fit: 512 inputs after the other, two such in LDS
+//
+// Measured, weights from memory: one row of 1024 to 151936 outputs in fp32 16.4 us, 4.95 TB/s, the rate of a
+// large copy; to 4096 outputs 3.0 us of kernel, 7 rows of 3072 to 1024 outputs 6.4, both the latency of
+// codes, products and join one after the other; 33 rows of 4096 to 16001 outputs in groups of 32 21.4 us,
+// where vector instructions (47 per 32 inputs of a tile, 6 of them products) are issued in half of the
+// cycles, LDS reads take a little less and 16 waves meet at a barrier every 512 inputs.
 // x through LDS also keeps the loads of weights ahead of their use: loads return in order, so one of x
 // behind them would wait for memory.
 #include <hip/hip_runtime.h>

@@ -211,3 +211,20 @@ def test_an_infinite_scale_stays_in_its_output(m, n, k, group):
     s[1::2] = float("inf")
     got = _linear(x.cuda(), q.cuda(), s.cuda(), z.cuda()).cpu()
     assert torch.equal(got[:, ::2], want[:, ::2]) and not torch.isfinite(got[:, 1::2]).any()
+
+
+@pytest.mark.parametrize("m,n", [(1, 100), (1, 5000), (12, 9000), (40, 5000), (40, 100)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_residual_in_place(m, n, dtype):
+    """The C entry point adds into out itself."""
+    from megaqwen_amd import _lib
+    k = 1152
+    q, s, z = (_cuda(t) for t in _weight(n, k, 64, torch.bfloat16, True, seed=12))
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).cuda()
+    r = torch.randn(m, n, generator=torch.Generator().manual_seed(10)).to(dtype).cuda()
+    want = _linear(x, q, s, z, residual=r, out_dtype=dtype)
+    _lib.check(_lib.load().mq_w4_linear(
+        x.data_ptr(), q.data_ptr(), s.data_ptr(), z.data_ptr(), r.data_ptr(), r.data_ptr(), m, n, k, 64, _lib.MQ_DTYPE_BF16,
+        _lib.MQ_DTYPE_BF16, _lib.MQ_DTYPE_BF16 if dtype == torch.bfloat16 else _lib.MQ_DTYPE_F32,
+        torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(r, want)
