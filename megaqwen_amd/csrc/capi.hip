@@ -712,10 +712,8 @@ int mq_w4_linear(const void* d_x, const void* d_qweight, const void* d_scales, c
   return launch_result(mq_launch_w4_linear(a, static_cast<hipStream_t>(stream)));
 }
 
-// Checks shared by the cache's entry points.  *run is false for an empty problem.
-static int check_kv4(const mq_kv4_cache* c, const int32_t* d_lengths, int t, MqKv4* out, bool* run) {
-  *run = false;
-  if (c == nullptr) return fail(MQ_ERR_INVALID_ARG, "cache is NULL");
+// Checks shared by the cache's entry points.
+static int check_kv4_sizes(const mq_kv4_cache* c, int t) {
   if (c->batch < 0 || c->kv_heads < 1 || c->max_seq < 1 || t < 0)
     return fail(MQ_ERR_INVALID_ARG, "bad size (batch %d, kv_heads %d, max_seq %d, t %d)", c->batch,
                 c->kv_heads, c->max_seq, t);
@@ -728,6 +726,15 @@ static int check_kv4(const mq_kv4_cache* c, const int32_t* d_lengths, int t, MqK
     return fail(MQ_ERR_INVALID_ARG, "group_size %d is not 32, 64 or 128, at most head_dim", g);
   if (c->batch > 65535 || (long long)t * c->kv_heads > (1 << 26))
     return fail(MQ_ERR_INVALID_ARG, "too many rows (batch %d, t %d, kv_heads %d)", c->batch, t, c->kv_heads);
+  return MQ_OK;
+}
+
+// *run is false for an empty problem.
+static int check_kv4(const mq_kv4_cache* c, const int32_t* d_lengths, int t, MqKv4* out, bool* run) {
+  *run = false;
+  if (c == nullptr) return fail(MQ_ERR_INVALID_ARG, "cache is NULL");
+  const int rc = check_kv4_sizes(c, t);
+  if (rc != MQ_OK) return rc;
   if (c->batch == 0 || t == 0) return MQ_OK;
   if (c->k_codes == nullptr || c->v_codes == nullptr || c->scales == nullptr || d_lengths == nullptr)
     return fail(MQ_ERR_INVALID_ARG, "NULL argument");
@@ -735,7 +742,7 @@ static int check_kv4(const mq_kv4_cache* c, const int32_t* d_lengths, int t, MqK
     return fail(MQ_ERR_INVALID_ARG, "codes must be 16-byte and scales 4-byte aligned");
   *out = MqKv4{static_cast<uint8_t*>(c->k_codes), static_cast<uint8_t*>(c->v_codes),
                static_cast<uint16_t*>(c->scales), d_lengths, c->batch, t, c->kv_heads, c->head_dim,
-               c->max_seq, g};
+               c->max_seq, c->group_size};
   *run = true;
   return MQ_OK;
 }
@@ -794,7 +801,7 @@ static int check_attend(const mq_kv4_cache* c, int t, int q_heads, int max_len) 
 }
 
 size_t mq_kv4_attend_workspace_bytes(const mq_kv4_cache* cache, int t, int q_heads, int max_len) {
-  if (cache == nullptr || cache->kv_heads < 1 || cache->kv_heads > 256 || cache->batch < 1 || t < 1 ||
+  if (cache == nullptr || cache->batch < 1 || t < 1 || check_kv4_sizes(cache, t) != MQ_OK ||
       check_attend(cache, t, q_heads, max_len) != MQ_OK)
     return 0;
   return mq_kv4_attend_workspace(cache->batch, t, q_heads, cache->kv_heads, cache->head_dim,

@@ -577,7 +577,7 @@ AtPlan at_plan(int B, int T, int Hq, int Hkv, int D, int G, int max_len) {
   return p;
 }
 
-int launched() { return hipGetLastError() == hipSuccess ? 0 : -1; }
+int launched() { return hipPeekAtLastError() == hipSuccess ? 0 : -1; }
 
 }  // namespace
 

@@ -413,5 +413,5 @@ int mq_launch_token_logprobs(const MqLogprobArgs& a, void* ws, hipStream_t strea
   if (a.type == 2) go(std::integral_constant<int, 2>());
   else if (a.type == 1) go(std::integral_constant<int, 1>());
   else go(std::integral_constant<int, 0>());
-  return hipGetLastError() == hipSuccess ? 0 : -1;
+  return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }

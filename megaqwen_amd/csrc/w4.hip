@@ -609,5 +609,5 @@ int mq_launch_w4_linear(const MqW4Args& a, hipStream_t stream) {
   };
   if (a.x_type == MQ_T_F16) pick(std::true_type());
   else pick(std::false_type());
-  return hipGetLastError() == hipSuccess ? 0 : -1;
+  return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }

@@ -111,3 +111,14 @@ def test_at_most_256_kv_heads():
     assert lib.mq_kv4_append(c, 4 * A, st, 5 * A, st, 6 * A, 1, _lib.MQ_DTYPE_BF16, None) == _lib.MQ_ERR_INVALID_ARG
     assert b"256" in lib.mq_last_error()
     assert lib.mq_kv4_read(c, 6 * A, 1, 4 * A, 5 * A, _lib.MQ_DTYPE_BF16, None) == _lib.MQ_ERR_INVALID_ARG
+
+
+def test_workspace_of_sizes_that_are_refused():
+    """0, and no arithmetic on them."""
+    lib, A = _lib.load(), 1 << 24
+    for kw in (dict(g=0), dict(g=-32), dict(g=48), dict(d=64, g=128), dict(d=0), dict(d=96), dict(h=0), dict(h=257), dict(b=0),
+               dict(b=70000), dict(n=0), dict(n=1 << 25)):
+        a = {**dict(b=1, h=4, n=32768, d=128, g=32), **kw}
+        c = ctypes.byref(_lib.Kv4Cache(A, 2 * A, 3 * A, a["b"], a["h"], a["n"], a["d"], a["g"]))
+        for t in (1, 0, -1, 1 << 30):
+            assert lib.mq_kv4_attend_workspace_bytes(c, t, 8, 32768) == 0, kw
