@@ -22,9 +22,10 @@
 //
 // Measured, weights from memory: one row of 1024 to 151936 outputs in fp32 16.4 us, 4.95 TB/s, the rate of a
 // large copy; to 4096 outputs 3.0 us of kernel, 7 rows of 3072 to 1024 outputs 6.4, both the latency of
-// codes, products and join one after the other; 33 rows of 4096 to 16001 outputs in groups of 32 21.4 us,
+// codes, products and join one after the other; 33 rows of 4096 to 16001 outputs in groups of 32 20 us,
 // where vector instructions (47 per 32 inputs of a tile, 6 of them products) are issued in half of the
-// cycles, LDS reads take a little less and 16 waves meet at a barrier every 512 inputs.
+// cycles, LDS reads take a little less and 16 waves meet at a barrier every 512 inputs.  (Its rows in an order
+// that no LDS read conflicts in: no faster, the writes or the loads of x take as much more.)
 // x through LDS also keeps the loads of weights ahead of their use: loads return in order, so one of x
 // behind them would wait for memory.
 #include <hip/hip_runtime.h>
@@ -167,13 +168,21 @@ template <int G, int U> struct W4Weights {
   }
 };
 
-// acc[t] += the products of a block whose first group is the first-th of sc (s16: all ones if the scales are
-// fp16, 0 for bf16); x_of(t, step) is the operand of row tile t.  AHEAD: a step's operands are read one step
+// acc[t] += the products of a block whose first group is the first-th of sc (fp16: its type; else bf16); x_of(t, step) is the operand of row tile t.  AHEAD: a step's operands are read one step
 // ahead, and no further: steps mixed by the scheduler take more registers than there are.
 template <bool F16, int G, int MT, bool ONE, bool AHEAD = true, class S, class X>
-MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const S& sc, int first, uint32_t s16, X x_of) {
+MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const S& sc, int first, bool fp16, X x_of) {
   constexpr int SPG = G / 32;            // steps of a group
   w4_exchange<G>(d);
+  // (a branch for all scales of the block at once; one per group moves all groups' sums behind the last)
+  float f[4 / SPG];
+  if (fp16) {
+#pragma unroll
+    for (int i = 0; i < 4 / SPG; ++i) f[i] = w4_from16(sc.scale(first + i) & 0xffffu, true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4 / SPG; ++i) f[i] = __uint_as_float(sc.scale(first + i) << 16);
+  }
   uint4 x[MT], zero;
   nb_f32x4 c[MT];
   if constexpr (AHEAD)
@@ -204,13 +213,10 @@ MQ_DEV void w4_block(nb_f32x4 (&acc)[MT], uint32_t (&d)[4], const S& sc, int fir
       c[t] = nb_mfma<F16>(x[t], w, c[t]);
     }
     if (s % SPG == SPG - 1) {
-      // (both readings and a select: a branch here moves all groups' sums to the end of the block)
-      const uint32_t sw = sc.scale(g), half = __float_as_uint(w4_from16(sw & 0xffffu, true));
-      const float f = __uint_as_float((half & s16) | ((sw << 16) & ~s16));
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int i = 0; i < (ONE ? 1 : 4); ++i) acc[t][i] = fmaf(f, c[t][i], acc[t][i]);
+        for (int i = 0; i < (ONE ? 1 : 4); ++i) acc[t][i] = fmaf(f[s / SPG], c[t][i], acc[t][i]);
 #pragma unroll
       for (int t = 0; t < MT; ++t) asm volatile("" : "+v"(acc[t]));      // (here, and not behind the next loads)
     }
@@ -281,7 +287,7 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
       y.x[s] = make_uint4(v[0], v[1], v[2], v[3]);
     }
   };
-  const uint32_t s16 = a.s_type == MQ_T_F16 ? ~0u : 0u;
+  const bool s16 = a.s_type == MQ_T_F16;
   nb_f32x4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
   Stretch y[U];
 #pragma unroll
@@ -371,7 +377,7 @@ __global__ void __launch_bounds__(W4_THREADS, MT == 2 ? 2 : G == 32 && !ONE ? 3 
   const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
   uint16_t* xs = (uint16_t*)lds;
   const Weights wt(a, (blockIdx.x * (pl.waves / pl.kw) + nw) * 16, pl.wide_scales, lane);
-  const uint32_t s16 = a.s_type == MQ_T_F16 ? ~0u : 0u;
+  const bool s16 = a.s_type == MQ_T_F16;
   uint32_t w[U][4];
   W4Scales<Weights::NS> sc;
 #pragma unroll
@@ -475,7 +481,7 @@ __global__ void __launch_bounds__(64 * W4_STRETCH_WAVES, 4) w4_stretch_kernel(Mq
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = wave / W4_STRETCH_KW, kw = wave % W4_STRETCH_KW;
   const int m0 = blockIdx.y * (16 * MT), rows = min(16 * MT, a.M - m0);
   const Weights wt(a, (blockIdx.x * W4_STRETCH_TILES + nw) * 16, lane);
-  const uint32_t s16 = a.s_type == MQ_T_F16 ? ~0u : 0u;
+  const bool s16 = a.s_type == MQ_T_F16;
   // A wave carries 64 pieces of rows wave, wave + 16, ..; rows that are not there are zeros.
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (size_t)m0 * a.K), (short)0, rows * a.K * 2, 0x00020000);
   uint16_t* const put = xs + wave * W4_STRETCH_ROW + (lane >> 4) * 128 + 8 * w4_slot<G>(lane & 15);
