@@ -21,7 +21,7 @@
 //   w4_stretch_kernel  the same where the rows do not fit: 512 inputs after the other, two such in LDS
 //
 // Measured, weights from memory: one row of 1024 to 151936 outputs in fp32 16.4 us, 4.95 TB/s, the rate of a
-// large copy; to 4096 outputs 3.0 us of kernel, 7 rows of 3072 to 1024 outputs 6.4, both the latency of
+// large copy; to 4096 outputs 3.0 us of kernel, 7 rows of 3072 to 1024 outputs 4.9, both the latency of
 // codes, products and join one after the other; 33 rows of 4096 to 16001 outputs in groups of 32 20 us,
 // where vector instructions (47 per 32 inputs of a tile, 6 of them products) are issued in half of the
 // cycles, LDS reads take a little less and 16 waves meet at a barrier every 512 inputs.  (Its rows in an order
@@ -88,7 +88,7 @@ template <int G> MQ_DEV int w4_slot(int piece) {
 }
 
 // Rows n0 .. n0 + rows of a tensor (in scalar registers)
-MQ_DEV int w4_outputs(const MqW4Args& a, int n0) { return __builtin_amdgcn_readfirstlane(max(0, min(16, a.N - n0))); }
+MQ_DEV int w4_outputs(const MqW4Args& a, int n0, int most = 16) { return __builtin_amdgcn_readfirstlane(max(0, min(most, a.N - n0))); }
 MQ_DEV __amdgpu_buffer_rsrc_t w4_rsrc(const void* p, int row_bytes, int n0, int rows) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)p + (size_t)n0 * row_bytes), (short)0, rows * row_bytes, 0x00020000);
 }
@@ -111,14 +111,14 @@ template <int G, int U> struct W4Weights {
   __amdgpu_buffer_rsrc_t wr, sr, zr;
   int K, groups, col, j;
   bool wide, zeros;
-  MQ_DEV W4Weights(const MqW4Args& a, int n0, bool wide_scales, int lane) {
+  MQ_DEV W4Weights(const MqW4Args& a, int n0, bool wide_scales, int lane, int outputs = 16) {     // (a power of two)
     K = a.K;
     groups = K / G;
-    col = lane & 15;
+    col = lane & (outputs - 1);
     j = lane >> 4;
     wide = wide_scales;
     zeros = a.zeros != nullptr;
-    const int rows = w4_outputs(a, n0);
+    const int rows = w4_outputs(a, n0, outputs);
     wr = w4_rsrc(a.qw, K / 2, n0, rows);
     sr = w4_rsrc(a.scales, groups * 2, n0, rows);
     zr = w4_rsrc(a.zeros, groups, n0, rows);
@@ -260,29 +260,33 @@ MQ_DEV void w4_finish(const MqW4Args& a, const nb_f32x4 (&acc)[MT], int m0, int 
   }
 }
 
-// 16 rows; wave w takes blocks w, w + 8, .. of the workgroup's 16 outputs.
+// 16 rows of the products, 2^slices slices of the inputs: row r is row r % R of x in slice r / R, R = 16 >>
+// slices, column c output c % R of the workgroup's R in slice c / R, and what counts of the result is where
+// the slices agree.  With few rows of x and few outputs that puts more compute units to work, each of which
+// has only so many loads in flight.  Wave w takes blocks w, w + 8, .. of every slice.
 template <bool F16, int G, bool ONE>
-__global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bool wide_scales) {
+__global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bool wide_scales, int slices) {
   constexpr int U = 3;                  // blocks in flight, with their pieces of x
   typedef W4Weights<G, 1> Weights;
   __shared__ float red[W4_WAVES * (ONE ? 1 : 4) * 64];
-  const int lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4, blocks = (a.K + 127) / 128;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Weights wt(a, blockIdx.x * 16, wide_scales, lane);
-  const int m0 = 16 * blockIdx.y, rows = min(16, a.M - m0);
+  const int lane = threadIdx.x & 63, col = lane & 15, j = lane >> 4;
+  const int shift = 4 - slices, R = 1 << shift, blocks = (((a.K + 127) / 128) + (1 << slices) - 1) >> slices;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), first = (col >> shift) * blocks;
+  const Weights wt(a, blockIdx.x * R, wide_scales, lane, R);
+  const int m0 = 16 * blockIdx.y, rows = min(R, a.M - m0);
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (size_t)m0 * a.K), (short)0, rows * a.K * 2, 0x00020000);
-  const int xrow = (ONE ? 0 : min(col, rows - 1)) * a.K;     // (rows past the last read it again)
+  const int xrow = (ONE ? 0 : min(col & (R - 1), rows - 1)) * a.K;     // (rows past the last read it again)
   struct Stretch {
     uint32_t w[4];
     W4Scales<Weights::NS> sc;
     uint4 x[4];
   };
   auto load = [&](Stretch& y, int b) {
-    wt.codes(y.w, b);
-    wt.scales(y.sc, b);
+    wt.codes(y.w, first + b);
+    wt.scales(y.sc, first + b);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const int k = 128 * b + 8 * w4_piece<G>(s, j);
+      const int k = 128 * (first + b) + 8 * w4_piece<G>(s, j);
       const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, k < a.K ? 2 * (xrow + k) : W4_FAR, 0, 0);
       y.x[s] = make_uint4(v[0], v[1], v[2], v[3]);
     }
@@ -294,9 +298,8 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
   for (int u = 0; u < U; ++u)
     if (wave + W4_WAVES * u < blocks) load(y[u], wave + W4_WAVES * u);
   // One output per thread at the end; its residual is on the way from here.
-  constexpr int R = ONE ? 1 : 4;
-  const int om = 4 * j + (wave & (R - 1)), on = 16 * blockIdx.x + col;
-  const bool mine = wave < R && om < rows && on < a.N;
+  const int ol = threadIdx.x & (R - 1), om = threadIdx.x >> shift, on = R * blockIdx.x + ol;
+  const bool mine = om < rows && on < a.N;
   const size_t out_at = (size_t)(m0 + om) * a.N + on;
   const float residual = mine && a.residual != nullptr ? w4_residual(a.residual, out_at, a.o_type) : 0.f;
   for (int b = wave; b < blocks; b += W4_WAVES * U) {
@@ -307,13 +310,17 @@ __global__ void __launch_bounds__(W4_THREADS, 4) w4_direct_kernel(MqW4Args a, bo
       if (b + W4_WAVES * (u + U) < blocks) load(y[u], b + W4_WAVES * (u + U));
     }
   }
+  constexpr int REGS = ONE ? 1 : 4;     // (one row is in register 0: R is 4 at least)
 #pragma unroll
-  for (int i = 0; i < R; ++i) red[(wave * R + i) * 64 + lane] = acc[0][i];
+  for (int i = 0; i < REGS; ++i) red[(wave * REGS + i) * 64 + lane] = acc[0][i];
   __syncthreads();
   if (!mine) return;
   float sum = 0.f;
+  for (int p = 0; p < 1 << slices; ++p) {
+    const int r = R * p + om, at = (r & 3) * 64 + (r >> 2) * 16 + R * p + ol;
 #pragma unroll
-  for (int q = 0; q < W4_WAVES; ++q) sum += red[(q * R + wave) * 64 + lane];
+    for (int q = 0; q < W4_WAVES; ++q) sum += red[q * REGS * 64 + at];
+  }
   w4_store(a.out, out_at, sum + residual, a.o_type);
 }
 
@@ -322,6 +329,7 @@ struct W4Plan {
   int mt;             // tiles of 16 rows
   int kw, waves;      // waves that split the inputs, waves of a workgroup
   int units;          // per wave: w4_unit() blocks each
+  int slices;         // w4_direct_kernel
   int lds;            // bytes
   bool wide_scales;   // the scales (and zeros) of a unit (or block, DIRECT) are whole, aligned loads
 };
@@ -540,6 +548,9 @@ __global__ void __launch_bounds__(64 * W4_STRETCH_WAVES, 4) w4_stretch_kernel(Mq
 //       16    8192 x 1024, 8192    5.3 25.1   6.2 23.3   |  12288 x 1024, 8192    7.3 35.6   6.3 32.1
 //       33    4096 x 1024, 8192    6.4 30.5   8.5 33.7   |   8192 x 1024, 8192   10.4 57.2   8.6 33.7
 //       64    2048 x 1024, 8192    5.1 23.6   9.6 35.0   |   4096 x 1024, 8192    8.6 45.1   9.8 38.2
+//    Its slices, 1, 2 and 4: as many as the rows leave room for while all workgroups are on the chip at once
+//    and a slice has 4 blocks, one row of 1024 outputs: 512 inputs 2.5 2.6 2.8, 1024 2.8 2.7 2.9, 3072 5.0 3.6
+//    3.3, 8192 8.9 6.0 4.4; 7 rows, 3072: 5.8 4.5.  (16 waves in place of 8, without slices: 5.7.)
 //  - WHOLE if two workgroups with all rows of x fit a compute unit: 60000 x 1024, groups of 32: 4 rows 12.2
 //    (STRETCH 13.5), 16 rows 14.1 (14.4), 32 rows 18.6 (23.3); 20000 x 2048: 4 rows 12.1 (14.2), 16 rows
 //    15.5 (14.9).
@@ -555,7 +566,11 @@ W4Plan w4_plan(const MqW4Args& a) {
   const int unit = p.kind == W4Plan::WHOLE ? W4_WHOLE_UNIT : 1;
   const int ns = unit * 128 / a.G;       // groups loaded at a time
   p.wide_scales = a.K % (ns * a.G) == 0 && ((uintptr_t)a.scales & 15) == 0 && ((uintptr_t)a.zeros & 15) == 0;
-  if (p.kind == W4Plan::DIRECT) return p;
+  if (p.kind == W4Plan::DIRECT) {
+    p.slices = 0;
+    while (p.slices < 2 && a.M <= (8 >> p.slices) && (tiles << (p.slices + 1)) <= 256 && (blocks >> (p.slices + 1)) >= 4) ++p.slices;
+    return p;
+  }
   if (p.kind == W4Plan::STRETCH) {
     p.waves = W4_STRETCH_WAVES;
     p.kw = W4_STRETCH_KW;
@@ -579,9 +594,10 @@ int mq_launch_w4_linear(const MqW4Args& a, hipStream_t stream) {
     constexpr bool F = decltype(f16)::value;
     constexpr int G = decltype(g)::value;
     if (p.kind == W4Plan::DIRECT) {
-      const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16);
-      if (a.M == 1) hipLaunchKernelGGL((w4_direct_kernel<F, G, true>), grid, dim3(W4_THREADS), 0, stream, a, p.wide_scales);
-      else hipLaunchKernelGGL((w4_direct_kernel<F, G, false>), grid, dim3(W4_THREADS), 0, stream, a, p.wide_scales);
+      const int outputs = 16 >> p.slices;
+      const dim3 grid((a.N + outputs - 1) / outputs, (a.M + 15) / 16);
+      if (a.M == 1) hipLaunchKernelGGL((w4_direct_kernel<F, G, true>), grid, dim3(W4_THREADS), 0, stream, a, p.wide_scales, p.slices);
+      else hipLaunchKernelGGL((w4_direct_kernel<F, G, false>), grid, dim3(W4_THREADS), 0, stream, a, p.wide_scales, p.slices);
       return;
     }
     for (int m0 = 0; m0 < a.M; m0 += 65535 * 64) {               // the grid's second dimension

@@ -228,3 +228,27 @@ def test_residual_in_place(m, n, dtype):
         _lib.MQ_DTYPE_BF16, _lib.MQ_DTYPE_BF16 if dtype == torch.bfloat16 else _lib.MQ_DTYPE_F32,
         torch.cuda.current_stream().cuda_stream))
     assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 5, 1024), (1, 70, 4096), (1, 1023, 8192), (2, 130, 2048), (3, 1030, 3072), (4, 9, 5120),
+                                   (5, 2050, 1024), (7, 900, 3072), (8, 31, 2048), (9, 31, 2048)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_few_outputs(m, n, k, group):
+    """Inputs of few outputs in slices, whole and with one group more or less than the slices hold."""
+    for k in (k, k + group, k - group):
+        q, s, z = _weight(n, k, group, torch.bfloat16, True, seed=m + n + k)
+        g = torch.Generator().manual_seed(12)
+        x, r = torch.randn(m, k, generator=g).to(torch.bfloat16), torch.randn(m, n, generator=g).to(torch.bfloat16)
+        _check(_linear(x.cuda(), q.cuda(), s.cuda(), z.cuda(), residual=r.cuda()), x, q, s, z, r, group)
+
+
+def test_non_finite_inputs_in_slices():
+    """As test_non_finite_inputs, where a product holds several slices of the inputs."""
+    q, s, z = _weight(40, 4096, 64, torch.bfloat16, True, seed=13)
+    x = torch.randn(4, 4096, generator=torch.Generator().manual_seed(13)).to(torch.bfloat16)
+    want = _linear(x.cuda(), q.cuda(), s.cuda(), z.cuda()).cpu()
+    x[2, 1500], s[7, 63], s[20, 0] = float("nan"), float("inf"), float("inf")
+    got = _linear(x.cuda(), q.cuda(), s.cuda(), z.cuda()).cpu()
+    keep = torch.ones(4, 40, dtype=torch.bool)
+    keep[2], keep[:, 7], keep[:, 20] = False, False, False
+    assert not torch.isfinite(got[~keep]).any() and torch.equal(got[keep], want[keep])
